@@ -363,6 +363,129 @@ int dsa_v32_topk_select(const float* scores, int64_t stride_row, const int32_t* 
 int dsa_v32_pack_fp8_rows(const float* latent, const void* rope_bf16, const int64_t* dst_rows, void* kv_rows_out,
                           int64_t num_rows, void* stream);
 
+/*
+ * ---- The front end: what lies between a layer's projections and the attention.  No counterpart in the reference lab, whose
+ * harness draws queries, caches and lists at random (common/host.cc:191-261).
+ *
+ * Rotation table: fp32 [max_positions, rope_dim], per position rope_dim / 2 cosines, then rope_dim / 2 sines.  A pair (a, b)
+ * becomes (a cos - b sin, a sin + b cos); pair i of a vector's rope_dim values is (2 i, 2 i + 1) when `interleaved`, else
+ * (i, i + rope_dim / 2).  A token whose position lies outside [0, max_positions) is a padding token: nothing is written for it.
+ * Norms are taken in fp32 over a whole vector: with `center` its mean is subtracted first, then x / sqrt(mean(x^2) + eps) *
+ * weight + bias; a NULL weight means no norm (and no centring), a NULL bias none.  Values are rounded once, at the end.
+ * e4m3 outputs: scale = amax / 448 (1 for a vector of zeros), value = e4m3(x / scale), as in dsa_v32_pack_fp8_rows.
+ */
+#define DSA_V32_DTYPE_BF16 0
+#define DSA_V32_DTYPE_FP32 1
+#define DSA_V32_DTYPE_E4M3 2
+
+/*
+ * Norm and rotation of the heads of queries and, in the same launch, of keys: rope_dim values from `rope_begin` on are
+ * rotated.  Out may be the input itself (same address and strides, bf16 in and out); otherwise they must not overlap.
+ * head_dim: a multiple of 8 up to 1024; rope_begin a multiple of 8, rope_dim of 16 (0: no rotation, positions may then be
+ * NULL).  Addresses of q, k and out and their strides are multiples of 16 bytes (8 for e4m3 out).
+ */
+typedef struct dsa_v32_norm_rotate_args {
+    const void* q;            /* [num_tokens, q_heads, head_dim], element strides below */
+    const void* k;            /* [num_tokens, k_heads, head_dim]; NULL with k_heads = 0 */
+    void* q_out;
+    void* k_out;
+    float* q_scale;           /* e4m3: [num_tokens, q_heads], times head_weight where that is given */
+    float* k_scale;           /* e4m3: [num_tokens, k_heads] */
+    const float* q_weight;    /* [head_dim] each */
+    const float* q_bias;
+    const float* k_weight;
+    const float* k_bias;
+    const float* head_weight; /* [num_tokens, q_heads] or NULL; e4m3 only */
+    const float* cos_sin;
+    const int32_t* positions; /* [num_tokens] */
+    int64_t stride_q_row, stride_q_head, stride_k_row, stride_k_head;
+    int64_t stride_qo_row, stride_qo_head, stride_ko_row, stride_ko_head;
+    int32_t num_tokens, q_heads, k_heads, head_dim;
+    int32_t rope_begin, rope_dim, max_positions;
+    int32_t in_dtype;         /* DSA_V32_DTYPE_BF16 or _FP32 */
+    int32_t out_dtype;        /* DSA_V32_DTYPE_BF16 or _E4M3 */
+    int32_t interleaved, center;
+    float eps;
+} dsa_v32_norm_rotate_args;
+int dsa_v32_norm_rotate(const dsa_v32_norm_rotate_args* args, void* stream);
+
+/*
+ * Index cache: what dsa_v32_index_scores reads of every position, DSA_V32_D_INDEX values.  bf16: rows of 128 values; fp8:
+ * pages of `page_block_size` positions, first the keys (128 e4m3 each), then their fp32 scales.  Its pages go by the same block
+ * table and physical rows as the attention's cache; page_block_size is a power of two from 16 on for it.
+ */
+#define DSA_V32_D_INDEX 128
+
+/*
+ * Appends tokens to the paged caches: token t is position positions[t] of sequence seq_ids[t] (seq_ids NULL: t / s_q).  Its
+ * row of the attention's cache is the normed latent (512 values) beside the rotated rope key (64 values); its row of the
+ * index cache the normed index key (128 values) whose first 64 are rotated.  Either cache may be left out (kv / index_cache
+ * NULL).  A token whose sequence is negative, whose position is outside the table, or whose row lies outside the cache (without a
+ * block table: outside its sequence's kv_batch_stride_rows rows, when those are not 0) is not written; no other byte of the caches changes.  A (sequence, position) may occur once in a call.  The rows of the inputs
+ * start on 16-byte boundaries.
+ */
+typedef struct dsa_v32_append_args {
+    const void* latent;        /* [num_tokens, 512], row stride below; in_dtype */
+    const void* rope;          /* [num_tokens, 64] */
+    const void* index_key;     /* [num_tokens, 128] */
+    void* kv;                  /* kv_dtype: rows of 1152 or 656 bytes */
+    void* index_cache;         /* the same type */
+    const float* latent_weight; /* [512] or NULL */
+    const float* index_weight; /* [128] or NULL */
+    const float* index_bias;
+    const float* cos_sin;      /* [max_positions, 64] */
+    const int32_t* positions;  /* [num_tokens] */
+    const int32_t* seq_ids;    /* [num_tokens] or NULL */
+    const int32_t* block_table;
+    int64_t stride_latent, stride_rope, stride_index_key;
+    int64_t num_kv_rows;       /* rows of either cache */
+    int64_t kv_batch_stride_rows;
+    int32_t num_tokens, s_q, num_seqs, block_table_stride, page_block_size, max_positions;
+    int32_t in_dtype, kv_dtype;
+    int32_t interleaved, index_interleaved, index_center;
+    float eps;
+} dsa_v32_append_args;
+int dsa_v32_append_cache(const dsa_v32_append_args* args, void* stream);
+
+/*
+ * Index scores: for query row q (of sequence q / s_q) and position p of its sequence
+ *     s[q, p] = key scale[p] * sum over heads h of weights[q, h] * max(0, q[q, h, :] . key[p, :])
+ * in fp32, and per block of `block` positions the largest of them (block 1: every score), as fp32
+ * [total_q, ceil(kv_len / block)] with row stride stride_o_row.  Only positions below valid_len[q] (NULL: kv_len) whose row
+ * lies inside the cache (and, as for the append, inside the sequence's rows) count; a block without any gets -inf, and every column is written.  A NaN score makes
+ * its block NaN.  q is e4m3 on an fp8 cache (its scales belong into the weights: q_scale of
+ * dsa_v32_norm_rotate), bf16 on a bf16 cache.  H <= 64; block is a power of two up to 128; page_block_size as for the index
+ * cache; without a block table kv_batch_stride_rows is a multiple of page_block_size.  q rows and heads start on 16-byte
+ * boundaries.  `status`: a device word that gets DSA_V32_ERR_DEVICE_WAIT when a bounded wait ran out, or NULL; the scores
+ * that were not computed are then NaN.
+ */
+typedef struct dsa_v32_index_scores_args {
+    const void* q;             /* [total_q, H, 128], element strides */
+    const float* weights;      /* [total_q, H], row stride in elements */
+    const void* index_cache;
+    const int32_t* valid_len;  /* [total_q] or NULL */
+    const int32_t* block_table;
+    float* out;
+    int32_t* status;
+    int64_t stride_q_row, stride_q_head, stride_w_row, stride_o_row;
+    int64_t num_index_rows;
+    int64_t kv_batch_stride_rows;
+    int32_t total_q, H, s_q, kv_len, block;
+    int32_t block_table_stride, page_block_size;
+    int32_t cache_dtype;       /* DSA_V32_KV_BF16 or DSA_V32_KV_FP8 */
+} dsa_v32_index_scores_args;
+int dsa_v32_index_scores(const dsa_v32_index_scores_args* args, void* stream);
+
+/*
+ * Selection of blocks: for every query row the `num_selected` blocks with the largest scores among those that hold one of the
+ * row's first valid_len[q] positions (NULL: all num_blocks * block), the first `first` of them and the last `local` ones always
+ * among the selected; written as the positions of the selected blocks below valid_len[q], ascending, -1 behind them:
+ * int32 [total_q, num_selected * block], the lists that the attention takes.  Ties go to the lower blocks, a NaN score is never
+ * preferred.  first + local <= num_selected.
+ */
+int dsa_v32_block_select(const float* scores, int64_t stride_row, const int32_t* valid_len, int32_t total_q, int32_t num_blocks,
+                         int32_t block, int32_t num_selected, int32_t first, int32_t local, int32_t* indices_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdsa_v32.so")
 
 D_QK, D_V, D_ROPE = 576, 512, 64
+D_INDEX = 128                       # values of an index key
 BF16_ROW_BYTES, FP8_ROW_BYTES = 1152, 656
 KV_BF16, KV_FP8 = 0, 1
 ERR_DEVICE_WAIT = 1001
@@ -58,6 +59,29 @@ class AttnArgs(C.Structure):
                 ("kv_dtype", C.c_int32), ("sm_scale", C.c_float)]
 
 
+class NormRotateArgs(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out", "q_scale", "k_scale", "q_weight", "q_bias", "k_weight", "k_bias", "head_weight",
+                                           "cos_sin", "positions")]
+                + [(n, C.c_int64) for n in ("stride_q_row", "stride_q_head", "stride_k_row", "stride_k_head", "stride_qo_row", "stride_qo_head",
+                                            "stride_ko_row", "stride_ko_head")]
+                + [(n, C.c_int32) for n in ("num_tokens", "q_heads", "k_heads", "head_dim", "rope_begin", "rope_dim", "max_positions", "in_dtype",
+                                            "out_dtype", "interleaved", "center")] + [("eps", C.c_float)])
+
+
+class AppendArgs(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("latent", "rope", "index_key", "kv", "index_cache", "latent_weight", "index_weight", "index_bias", "cos_sin",
+                                           "positions", "seq_ids", "block_table")]
+                + [(n, C.c_int64) for n in ("stride_latent", "stride_rope", "stride_index_key", "num_kv_rows", "kv_batch_stride_rows")]
+                + [(n, C.c_int32) for n in ("num_tokens", "s_q", "num_seqs", "block_table_stride", "page_block_size", "max_positions", "in_dtype",
+                                            "kv_dtype", "interleaved", "index_interleaved", "index_center")] + [("eps", C.c_float)])
+
+
+class IndexScoresArgs(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "weights", "index_cache", "valid_len", "block_table", "out", "status")]
+                + [(n, C.c_int64) for n in ("stride_q_row", "stride_q_head", "stride_w_row", "stride_o_row", "num_index_rows", "kv_batch_stride_rows")]
+                + [(n, C.c_int32) for n in ("total_q", "H", "s_q", "kv_len", "block", "block_table_stride", "page_block_size", "cache_dtype")])
+
+
 class HostIO(C.Structure):
     _fields_ = [("q_host", C.c_void_p), ("indices_host", C.c_void_p), ("out_host", C.c_void_p),
                 ("lse_host", C.c_void_p), ("q_bytes", C.c_int64), ("out_bytes", C.c_int64)]
@@ -67,7 +91,8 @@ EXPORTS = ["dsa_v32_abi_version", "dsa_v32_error_string", "dsa_v32_plan_info_get
            "dsa_v32_plan_host", "dsa_v32_plan_read", "dsa_v32_plan_release", "dsa_v32_decode_bf16", "dsa_v32_decode_fp8",
            "dsa_v32_prefill_bf16", "dsa_v32_combine", "dsa_v32_decode_pipeline", "dsa_v32_device_status",
            "dsa_v32_debug_rows", "dsa_v32_pack_fp8_rows", "dsa_v32_decode_pipeline_host",
-           "dsa_v32_decode_pipeline_static", "dsa_v32_static_scratch_address", "dsa_v32_selftest_wait_expiry", "dsa_v32_decode_pipeline_allgather", "dsa_v32_ipc_export", "dsa_v32_ipc_open", "dsa_v32_ipc_close", "dsa_v32_decode_pipeline_host_chunked", "dsa_v32_decode_pipeline_host_lanes", "dsa_v32_decode_pipeline_v4", "dsa_v32_topk_select"]
+           "dsa_v32_decode_pipeline_static", "dsa_v32_static_scratch_address", "dsa_v32_selftest_wait_expiry", "dsa_v32_decode_pipeline_allgather", "dsa_v32_ipc_export", "dsa_v32_ipc_open", "dsa_v32_ipc_close", "dsa_v32_decode_pipeline_host_chunked", "dsa_v32_decode_pipeline_host_lanes", "dsa_v32_decode_pipeline_v4", "dsa_v32_topk_select",
+           "dsa_v32_norm_rotate", "dsa_v32_append_cache", "dsa_v32_index_scores", "dsa_v32_block_select"]
 
 _lib = None
 
@@ -114,6 +139,10 @@ def lib():
         L.dsa_v32_debug_rows.argtypes = [C.POINTER(AttnArgs), C.c_void_p, C.c_void_p]
         L.dsa_v32_topk_select.argtypes = [C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]
         L.dsa_v32_pack_fp8_rows.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
+        L.dsa_v32_norm_rotate.argtypes = [C.POINTER(NormRotateArgs), C.c_void_p]
+        L.dsa_v32_append_cache.argtypes = [C.POINTER(AppendArgs), C.c_void_p]
+        L.dsa_v32_index_scores.argtypes = [C.POINTER(IndexScoresArgs), C.c_void_p]
+        L.dsa_v32_block_select.argtypes = [C.c_void_p, C.c_int64, C.c_void_p] + [C.c_int32] * 6 + [C.c_void_p, C.c_void_p]
         _lib = L
     return _lib
 
@@ -371,3 +400,176 @@ def mla_decode_launch_pipeline_static(q, kv, indices, sm_scale, *, s_q=1, block_
         a.workspace = lib().dsa_v32_static_scratch_address()
         _check(lib().dsa_v32_device_status(C.byref(a), _stream()), "dsa_v32_device_status")
     return out, lse
+
+
+# ------------------------------------------------------------------ the front end: from a layer's projections to the attention's lists
+DTYPE_BF16, DTYPE_FP32, DTYPE_E4M3 = 0, 1, 2
+_IN_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_FP32}
+_OUT_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float8_e4m3fn: DTYPE_E4M3}
+
+
+def _here(*tensors):
+    """All tensors live on the current device: the launch goes to its current stream."""
+    dev = torch._C._cuda_getDevice()
+    for t in tensors:
+        assert t is None or t.get_device() == dev, "a tensor is not on the current device"
+
+
+def _vec(t, n, dtype=torch.float32):
+    """Address of a dense vector of n values, or None."""
+    if t is None:
+        return None
+    assert t.dtype == dtype and t.numel() == n and t.is_contiguous()
+    return t.data_ptr()
+
+
+def norm_rotate(q, cos_sin, positions, *, k=None, q_weight=None, k_weight=None, q_bias=None, k_bias=None, center=False, eps=1e-6, rope_begin=0,
+                interleaved=True, head_weight=None, out_dtype=torch.bfloat16, q_out=None, k_out=None, q_scale=None, k_scale=None):
+    """Norm (with a weight; `center`: of the values less their mean) and rotation of every head of q [tokens, heads, dim] and, in the
+    same launch, k; bf16 or fp32 in, bf16 or float8_e4m3fn out.
+
+    cos_sin fp32 [positions, rope_dim]: rope_dim / 2 cosines, then as many sines; None: no rotation.  The rope_dim values from rope_begin
+    on are rotated in pairs (2 i, 2 i + 1), or (i, i + rope_dim / 2) when not `interleaved`.  positions int32 [tokens]: nothing is written for
+    one outside the table (padding).  e4m3 out: each head's values over its scale amax / 448; q's scales are multiplied by
+    head_weight [tokens, heads].  q_out may be q.  Returns (q_out, k_out, q_scale, k_scale), None where there is none."""
+    if q_out is not None:
+        out_dtype = q_out.dtype
+    T, H, D = q.shape
+    assert q.dtype in _IN_DTYPES and out_dtype in _OUT_DTYPES and (D == 1 or q.stride(2) == 1)
+    e4m3 = out_dtype == torch.float8_e4m3fn
+    Hk = 0
+    if k is not None:
+        Hk = k.shape[1]
+        assert k.dtype == q.dtype and k.shape == (T, Hk, D) and Hk > 0 and k.stride(2) == 1
+        if k_out is None:
+            k_out = torch.empty(T, Hk, D, dtype=out_dtype, device=q.device)
+        assert k_out.dtype == out_dtype and k_out.shape == k.shape and k_out.stride(2) == 1
+    else:
+        assert k_out is None and k_weight is None and k_bias is None and k_scale is None
+    if q_out is None:
+        q_out = torch.empty(T, H, D, dtype=out_dtype, device=q.device)
+    assert q_out.shape == q.shape and q_out.stride(2) == 1
+    if e4m3:
+        if q_scale is None:
+            q_scale = torch.empty(T, H, dtype=torch.float32, device=q.device)
+        if Hk and k_scale is None:
+            k_scale = torch.empty(T, Hk, dtype=torch.float32, device=q.device)
+    else:
+        assert q_scale is None and k_scale is None and head_weight is None
+    _here(q, k, q_out, k_out, q_scale, k_scale, q_weight, q_bias, k_weight, k_bias, head_weight, cos_sin, positions)
+    R = P = 0
+    if cos_sin is not None:
+        assert cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.is_contiguous() and positions is not None
+        P, R = cos_sin.shape
+    elif positions is not None:
+        P = 0x7FFFFFFF      # no table: every position from 0 on
+    qs, qo = q.stride(), q_out.stride()
+    ks, ko = (k.stride(), k_out.stride()) if Hk else ((0, 0), (0, 0))
+    a = NormRotateArgs(q.data_ptr(), k.data_ptr() if Hk else None, q_out.data_ptr(), k_out.data_ptr() if Hk else None, _vec(q_scale, T * H),
+                       _vec(k_scale, T * Hk), _vec(q_weight, D), _vec(q_bias, D), _vec(k_weight, D), _vec(k_bias, D), _vec(head_weight, T * H),
+                       cos_sin.data_ptr() if R else None, _vec(positions, T, torch.int32), qs[0], qs[1], ks[0], ks[1], qo[0], qo[1], ko[0], ko[1],
+                       T, H, Hk, D, rope_begin, R, P, _IN_DTYPES[q.dtype], _OUT_DTYPES[out_dtype], 1 if interleaved else 0, 1 if center else 0, eps)
+    _check(lib().dsa_v32_norm_rotate(C.byref(a), _stream()), "dsa_v32_norm_rotate")
+    return q_out, k_out, q_scale, k_scale
+
+
+def index_cache_pages(num_pages, fp8, page_block_size=64, device="cuda"):
+    """An index cache of zeros: uint8 [pages, page * 132] (per page its keys, then their scales) or bf16 [pages * page, 128]."""
+    if fp8:
+        return torch.zeros(num_pages, page_block_size * (D_INDEX + 4), dtype=torch.uint8, device=device)
+    return torch.zeros(num_pages * page_block_size, D_INDEX, dtype=torch.bfloat16, device=device)
+
+
+def _index_rows(cache, page_block_size):
+    """(type, rows) of an index cache."""
+    assert cache.is_contiguous() and cache.dim() == 2
+    if cache.dtype == torch.uint8:
+        assert cache.shape[1] == page_block_size * (D_INDEX + 4)
+        return KV_FP8, cache.shape[0] * page_block_size
+    assert cache.dtype == torch.bfloat16 and cache.shape[1] == D_INDEX
+    return KV_BF16, cache.shape[0]
+
+
+def _table(block_table):
+    if block_table is None:
+        return None, 0, 0
+    assert block_table.dtype == torch.int32 and block_table.is_contiguous() and block_table.dim() == 2
+    return block_table.data_ptr(), block_table.shape[0], block_table.shape[1]
+
+
+def append_cache(latent, rope, kv, cos_sin, positions, *, seq_ids=None, s_q=1, block_table=None, page_block_size=64, kv_batch_stride_rows=0,
+                 latent_weight=None, index_key=None, index_cache=None, index_weight=None, index_bias=None, index_center=False, eps=1e-6,
+                 interleaved=True, index_interleaved=None):
+    """Appends tokens to the paged caches in one launch: latent [tokens, 512] (RMS norm when latent_weight is given) and rope [tokens, 64]
+    (rotated) to rows of kv (bf16 [rows, 576] or uint8 [rows, 656]), index_key [tokens, 128] (norm when index_weight is given, its first 64
+    values rotated) to index_cache of the same type (index_cache_pages).  bf16 or fp32 in.  Token t is position positions[t] of sequence
+    seq_ids[t] (None: t // s_q); a negative sequence, a position outside cos_sin [positions, 64] or a row outside the cache writes nothing.
+    latent = rope = kv = None: the index cache alone."""
+    tokens = positions.shape[0]
+    x = latent if latent is not None else index_key
+    assert x is not None and x.dtype in _IN_DTYPES
+    assert cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.shape[1] == D_ROPE and cos_sin.is_contiguous()
+    _here(latent, rope, kv, cos_sin, positions, seq_ids, block_table, latent_weight, index_key, index_cache, index_weight, index_bias)
+    kinds = []
+    if kv is not None:
+        assert latent.shape == (tokens, D_V) and rope.shape == (tokens, D_ROPE) and rope.dtype == x.dtype and latent.stride(1) == 1 and rope.stride(1) == 1
+        assert kv.is_contiguous() and (kv.dtype, kv.shape[-1]) in ((torch.uint8, FP8_ROW_BYTES), (torch.bfloat16, D_QK))
+        kinds.append((KV_FP8 if kv.dtype == torch.uint8 else KV_BF16, kv.numel() // kv.shape[-1]))
+    else:
+        assert latent is None and rope is None and latent_weight is None
+    if index_cache is not None:
+        assert index_key.shape == (tokens, D_INDEX) and index_key.dtype == x.dtype and index_key.stride(1) == 1
+        kinds.append(_index_rows(index_cache, page_block_size))
+    else:
+        assert index_key is None and index_weight is None and index_bias is None
+    assert len(kinds) == 1 or kinds[0] == kinds[1], "the two caches have different types or rows"
+    table, num_seqs, table_stride = _table(block_table)
+    a = AppendArgs(latent.data_ptr() if kv is not None else None, rope.data_ptr() if kv is not None else None,
+                   index_key.data_ptr() if index_cache is not None else None, kv.data_ptr() if kv is not None else None,
+                   index_cache.data_ptr() if index_cache is not None else None, _vec(latent_weight, D_V), _vec(index_weight, D_INDEX),
+                   _vec(index_bias, D_INDEX), cos_sin.data_ptr(), _vec(positions, tokens, torch.int32), _vec(seq_ids, tokens, torch.int32), table,
+                   latent.stride(0) if kv is not None else 0, rope.stride(0) if kv is not None else 0,
+                   index_key.stride(0) if index_cache is not None else 0, kinds[0][1], kv_batch_stride_rows, tokens, s_q, num_seqs, table_stride,
+                   page_block_size, cos_sin.shape[0], _IN_DTYPES[x.dtype], kinds[0][0], 1 if interleaved else 0,
+                   1 if (interleaved if index_interleaved is None else index_interleaved) else 0, 1 if index_center else 0, eps)
+    _check(lib().dsa_v32_append_cache(C.byref(a), _stream()), "dsa_v32_append_cache")
+
+
+def index_scores(q, weights, index_cache, valid_len, kv_len, *, s_q=1, block=1, block_table=None, page_block_size=64, kv_batch_stride_rows=0, out=None,
+                 status=None):
+    """Index scores of the first kv_len positions of every query row's sequence (row // s_q), the largest of each block of `block` positions:
+    sum over heads of weights * max(0, q . key), times the key's scale on an fp8 cache; -inf where no position below valid_len [rows] lies.
+
+    q [rows, H, 128], float8_e4m3fn on an fp8 cache, bf16 on a bf16 one; weights fp32 [rows, H] (on an fp8 cache with q's scales in them:
+    norm_rotate's head_weight).  Returns fp32 [rows, ceil(kv_len / block)], which topk_select (block 1) and block_select take.
+    status: int32 [1], gets ERR_DEVICE_WAIT where a bounded wait in the kernel ran out (the scores are then NaN)."""
+    total_q, H, D = q.shape
+    kind, rows = _index_rows(index_cache, page_block_size)
+    assert D == D_INDEX and q.stride(2) == 1 and q.dtype == (torch.float8_e4m3fn if kind == KV_FP8 else torch.bfloat16)
+    assert weights.dtype == torch.float32 and weights.shape == (total_q, H) and (H == 1 or weights.stride(1) == 1)
+    cols = -(-kv_len // block)
+    if out is None:
+        out = torch.empty(total_q, cols, dtype=torch.float32, device=q.device)
+    assert out.dtype == torch.float32 and out.shape == (total_q, cols) and (cols == 1 or out.stride(1) == 1)
+    _here(q, weights, index_cache, valid_len, block_table, out, status)
+    table, num_seqs, table_stride = _table(block_table)
+    assert table is None or num_seqs * s_q >= total_q, "the block table has fewer rows than there are sequences"
+    a = IndexScoresArgs(q.data_ptr(), weights.data_ptr(), index_cache.data_ptr(), _vec(valid_len, total_q, torch.int32), table, out.data_ptr(),
+                        _vec(status, 1, torch.int32), q.stride(0), q.stride(1), weights.stride(0), out.stride(0), rows, kv_batch_stride_rows,
+                        total_q, H, s_q, kv_len, block, table_stride, page_block_size, kind)
+    _check(lib().dsa_v32_index_scores(C.byref(a), _stream()), "dsa_v32_index_scores")
+    return out
+
+
+def block_select(scores, num_selected, block, valid_len=None, *, first=0, local=0, out=None):
+    """scores fp32 [rows, blocks] (index_scores) -> int32 [rows, num_selected * block]: the positions below valid_len [rows] (None: all) of
+    the num_selected best blocks of every row, the first `first` and last `local` ones always among them; ascending, -1 padded."""
+    assert scores.dtype == torch.float32 and scores.dim() == 2 and (scores.shape[1] == 1 or scores.stride(1) == 1)
+    rows, blocks = scores.shape
+    if out is None:
+        out = torch.empty(rows, num_selected * block, dtype=torch.int32, device=scores.device)
+    assert out.dtype == torch.int32 and out.shape == (rows, num_selected * block) and out.is_contiguous()
+    _here(scores, valid_len, out)
+    _check(lib().dsa_v32_block_select(scores.data_ptr(), scores.stride(0) if rows > 1 else blocks, _vec(valid_len, rows, torch.int32), rows, blocks, block,
+                                      num_selected, first, local, out.data_ptr(), _stream()), "dsa_v32_block_select")
+    return out

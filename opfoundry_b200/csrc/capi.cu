@@ -8,6 +8,7 @@
 #include <mutex>
 #include <vector>
 #include "defs.h"
+#include "front.h"
 #include "plan.h"
 #include "tmap.h"
 
@@ -868,6 +869,110 @@ int dsa_v32_pack_fp8_rows(const float* latent, const void* rope_bf16, const int6
     if (!aligned16(latent) || (reinterpret_cast<uintptr_t>(rope_bf16) & 3u) || (reinterpret_cast<uintptr_t>(kv_rows_out) & 3u))
         return DSA_V32_ERR_ALIGN;
     cudaError_t e = launch_pack_fp8(latent, rope_bf16, dst_rows, kv_rows_out, num_rows, (cudaStream_t)stream);
+    return e == cudaSuccess ? DSA_V32_OK : (int)e;
+}
+
+// ------------------------------------------------------------------ the front end
+namespace {
+bool misaligned(const void* p, uintptr_t mask) { return (reinterpret_cast<uintptr_t>(p) & mask) != 0; }
+
+// heads that do not overlap, rows likewise; a stride that no element uses may be anything
+bool strides_ok(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t dim) {
+    return (heads <= 1 || head >= dim) && (rows <= 1 || row >= (heads - 1) * (heads > 1 ? head : 0) + dim);
+}
+bool strides_aligned(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t unit) {
+    return (heads <= 1 || head % unit == 0) && (rows <= 1 || row % unit == 0);
+}
+// pages of an index cache: whole pages of a tile, or a tile of whole pages
+bool index_page_ok(int page) { return page >= 16 && (page & (page - 1)) == 0; }
+}  // namespace
+
+int dsa_v32_norm_rotate(const dsa_v32_norm_rotate_args* a, void* stream) {
+    if (!a) return DSA_V32_ERR_NULL;
+    if (a->num_tokens < 0 || a->q_heads <= 0 || a->k_heads < 0 || a->head_dim <= 0 || a->head_dim > 1024 || a->head_dim % 8) return DSA_V32_ERR_SHAPE;
+    if (a->in_dtype != DSA_V32_DTYPE_BF16 && a->in_dtype != DSA_V32_DTYPE_FP32) return DSA_V32_ERR_DTYPE;
+    if (a->out_dtype != DSA_V32_DTYPE_BF16 && a->out_dtype != DSA_V32_DTYPE_E4M3) return DSA_V32_ERR_DTYPE;
+    const bool e4m3 = a->out_dtype == DSA_V32_DTYPE_E4M3;
+    if (a->rope_dim < 0 || a->rope_dim % 16 || a->rope_begin < 0 || a->rope_begin % 8 || a->rope_begin > a->head_dim - a->rope_dim) return DSA_V32_ERR_SHAPE;
+    if (a->positions && a->max_positions <= 0) return DSA_V32_ERR_SHAPE;
+    if (!(a->eps >= 0.0f) || !std::isfinite(a->eps)) return DSA_V32_ERR_SHAPE;
+    if (a->num_tokens == 0) return DSA_V32_OK;
+    if (!a->q || !a->q_out || (a->k_heads > 0 && (!a->k || !a->k_out))) return DSA_V32_ERR_NULL;
+    if (a->rope_dim > 0 && (!a->cos_sin || !a->positions)) return DSA_V32_ERR_NULL;
+    if (e4m3 && (!a->q_scale || (a->k_heads > 0 && !a->k_scale))) return DSA_V32_ERR_NULL;
+    if (!e4m3 && a->head_weight) return DSA_V32_ERR_DTYPE;
+    const int64_t in_unit = a->in_dtype == DSA_V32_DTYPE_FP32 ? 4 : 8, d = a->head_dim;
+    struct Side { const void *x, *out; const float *w, *b; int64_t row, head, o_row, o_head, heads; };
+    const Side sides[2] = {{a->q, a->q_out, a->q_weight, a->q_bias, a->stride_q_row, a->stride_q_head, a->stride_qo_row, a->stride_qo_head, a->q_heads},
+                           {a->k, a->k_out, a->k_weight, a->k_bias, a->stride_k_row, a->stride_k_head, a->stride_ko_row, a->stride_ko_head, a->k_heads}};
+    for (const Side& s : sides) {
+        if (s.heads == 0) continue;
+        if (s.b && !s.w) return DSA_V32_ERR_NULL;
+        if (!strides_ok(a->num_tokens, s.row, s.heads, s.head, d) || !strides_ok(a->num_tokens, s.o_row, s.heads, s.o_head, d)) return DSA_V32_ERR_SHAPE;
+        if (!aligned16(s.x) || misaligned(s.out, e4m3 ? 7 : 15) || misaligned(s.w, 15) || misaligned(s.b, 15)) return DSA_V32_ERR_ALIGN;
+        if (!strides_aligned(a->num_tokens, s.row, s.heads, s.head, in_unit) || !strides_aligned(a->num_tokens, s.o_row, s.heads, s.o_head, 8)) return DSA_V32_ERR_ALIGN;
+    }
+    if (misaligned(a->cos_sin, 15)) return DSA_V32_ERR_ALIGN;
+    cudaError_t e = launch_norm_rotate(*a, (cudaStream_t)stream);
+    return e == cudaSuccess ? DSA_V32_OK : (int)e;
+}
+
+int dsa_v32_append_cache(const dsa_v32_append_args* a, void* stream) {
+    if (!a) return DSA_V32_ERR_NULL;
+    if (a->in_dtype != DSA_V32_DTYPE_BF16 && a->in_dtype != DSA_V32_DTYPE_FP32) return DSA_V32_ERR_DTYPE;
+    if (a->kv_dtype != DSA_V32_KV_BF16 && a->kv_dtype != DSA_V32_KV_FP8) return DSA_V32_ERR_DTYPE;
+    if (!a->kv && !a->index_cache) return DSA_V32_ERR_NULL;
+    if (a->num_tokens < 0 || (!a->seq_ids && a->s_q <= 0) || a->max_positions <= 0 || a->num_seqs < 0) return DSA_V32_ERR_SHAPE;
+    if (a->num_kv_rows <= 0 || a->num_kv_rows >= (int64_t(1) << 31) - 1 || a->page_block_size <= 0) return DSA_V32_ERR_SHAPE;
+    if (a->block_table ? a->block_table_stride <= 0 : a->kv_batch_stride_rows < 0) return DSA_V32_ERR_SHAPE;
+    if (a->index_cache && !index_page_ok(a->page_block_size)) return DSA_V32_ERR_SHAPE;
+    if (!(a->eps >= 0.0f) || !std::isfinite(a->eps)) return DSA_V32_ERR_SHAPE;
+    if (a->num_tokens == 0) return DSA_V32_OK;
+    if (!a->positions || !a->cos_sin || (a->kv && (!a->latent || !a->rope)) || (a->index_cache && !a->index_key)) return DSA_V32_ERR_NULL;
+    if (a->index_bias && !a->index_weight) return DSA_V32_ERR_NULL;
+    const int64_t unit = a->in_dtype == DSA_V32_DTYPE_FP32 ? 4 : 8;
+    if (a->kv) {
+        if (!strides_ok(a->num_tokens, a->stride_latent, 1, 0, kDV) || !strides_ok(a->num_tokens, a->stride_rope, 1, 0, kDRope)) return DSA_V32_ERR_SHAPE;
+        if (!aligned16(a->latent) || !aligned16(a->rope) || !aligned16(a->kv) || misaligned(a->latent_weight, 15)) return DSA_V32_ERR_ALIGN;
+        if (!strides_aligned(a->num_tokens, a->stride_latent, 1, 0, unit) || !strides_aligned(a->num_tokens, a->stride_rope, 1, 0, unit)) return DSA_V32_ERR_ALIGN;
+    }
+    if (a->index_cache) {
+        if (!strides_ok(a->num_tokens, a->stride_index_key, 1, 0, kDIndex)) return DSA_V32_ERR_SHAPE;
+        if (!aligned16(a->index_key) || !aligned16(a->index_cache) || misaligned(a->index_weight, 15) || misaligned(a->index_bias, 15)) return DSA_V32_ERR_ALIGN;
+        if (!strides_aligned(a->num_tokens, a->stride_index_key, 1, 0, unit)) return DSA_V32_ERR_ALIGN;
+    }
+    if (!aligned16(a->cos_sin)) return DSA_V32_ERR_ALIGN;
+    cudaError_t e = launch_append(*a, (cudaStream_t)stream);
+    return e == cudaSuccess ? DSA_V32_OK : (int)e;
+}
+
+int dsa_v32_index_scores(const dsa_v32_index_scores_args* a, void* stream) {
+    if (!a) return DSA_V32_ERR_NULL;
+    if (a->cache_dtype != DSA_V32_KV_BF16 && a->cache_dtype != DSA_V32_KV_FP8) return DSA_V32_ERR_DTYPE;
+    if (a->total_q < 0 || a->s_q <= 0 || a->total_q % a->s_q || a->H <= 0 || a->H > 64 || a->kv_len <= 0) return DSA_V32_ERR_SHAPE;
+    if (a->kv_len > 0x7FFFFFFF - 256) return DSA_V32_ERR_SHAPE;   // positions of a tile behind it stay 32-bit numbers
+    if (a->block <= 0 || a->block > 128 || (a->block & (a->block - 1))) return DSA_V32_ERR_SHAPE;
+    if (!index_page_ok(a->page_block_size)) return DSA_V32_ERR_SHAPE;
+    if (a->num_index_rows <= 0 || a->num_index_rows >= (int64_t(1) << 31) - 1 || a->num_index_rows % a->page_block_size) return DSA_V32_ERR_SHAPE;
+    if (a->block_table ? a->block_table_stride <= 0 : (a->kv_batch_stride_rows < 0 || a->kv_batch_stride_rows % a->page_block_size)) return DSA_V32_ERR_SHAPE;
+    if (a->total_q == 0) return DSA_V32_OK;
+    if (!a->q || !a->weights || !a->index_cache || !a->out) return DSA_V32_ERR_NULL;
+    const int64_t unit = a->cache_dtype == DSA_V32_KV_FP8 ? 16 : 8;
+    if (!strides_ok(a->total_q, a->stride_q_row, a->H, a->stride_q_head, kDIndex)) return DSA_V32_ERR_SHAPE;
+    if (a->total_q > 1 && (a->stride_w_row < a->H || a->stride_o_row < (a->kv_len + a->block - 1) / a->block)) return DSA_V32_ERR_SHAPE;
+    if (!aligned16(a->q) || !aligned16(a->index_cache) || !strides_aligned(a->total_q, a->stride_q_row, a->H, a->stride_q_head, unit)) return DSA_V32_ERR_ALIGN;
+    if (misaligned(a->weights, 3) || misaligned(a->out, 3)) return DSA_V32_ERR_ALIGN;
+    cudaError_t e = launch_index_scores(*a, (cudaStream_t)stream);
+    return e == cudaSuccess ? DSA_V32_OK : (int)e;
+}
+
+int dsa_v32_block_select(const float* scores, int64_t stride_row, const int32_t* valid_len, int32_t total_q, int32_t num_blocks, int32_t block,
+                         int32_t num_selected, int32_t first, int32_t local, int32_t* indices_out, void* stream) {
+    if (!scores || !indices_out) return DSA_V32_ERR_NULL;
+    if (total_q < 0 || num_blocks <= 0 || block <= 0 || num_selected <= 0 || stride_row < num_blocks) return DSA_V32_ERR_SHAPE;
+    if (first < 0 || local < 0 || first > num_selected - local) return DSA_V32_ERR_SHAPE;
+    if ((int64_t)num_blocks * block >= (int64_t(1) << 31) || (int64_t)num_selected * block >= (int64_t(1) << 31)) return DSA_V32_ERR_SHAPE;
+    cudaError_t e = launch_block_select(scores, stride_row, valid_len, total_q, num_blocks, block, num_selected, first, local, indices_out, (cudaStream_t)stream);
     return e == cudaSuccess ? DSA_V32_OK : (int)e;
 }
 
