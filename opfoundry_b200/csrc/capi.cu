@@ -962,7 +962,19 @@ int dsa_v32_index_scores(const dsa_v32_index_scores_args* a, void* stream) {
     if (a->total_q > 1 && (a->stride_w_row < a->H || a->stride_o_row < (a->kv_len + a->block - 1) / a->block)) return DSA_V32_ERR_SHAPE;
     if (!aligned16(a->q) || !aligned16(a->index_cache) || !strides_aligned(a->total_q, a->stride_q_row, a->H, a->stride_q_head, unit)) return DSA_V32_ERR_ALIGN;
     if (misaligned(a->weights, 3) || misaligned(a->out, 3)) return DSA_V32_ERR_ALIGN;
-    cudaError_t e = launch_index_scores(*a, (cudaStream_t)stream);
+    // 16-byte rows of keys and heads: 128 bytes of a key and of a head are one row of a box
+    const bool fp8 = a->cache_dtype == DSA_V32_KV_FP8;
+    const uint64_t bytes = fp8 ? 1 : 2, page = uint64_t(a->page_block_size);
+    const CUtensorMapDataType type = fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const int64_t head = a->H > 1 ? a->stride_q_head : kDIndex, row = a->total_q > 1 ? a->stride_q_row : head * a->H;   // (a stride that nothing uses may be anything)
+    const uint64_t kdims[3] = {uint64_t(kDIndex), page, uint64_t(a->num_index_rows) / page}, kstr[2] = {kDIndex * bytes, page * (fp8 ? kDIndex + 4 : 2 * kDIndex)};
+    const uint32_t kbox[3] = {uint32_t(128 / bytes), uint32_t(page < 128 ? page : 128), 1};
+    const uint64_t qdims[3] = {uint64_t(kDIndex), uint64_t(a->H), uint64_t(a->total_q)}, qstr[2] = {uint64_t(head) * bytes, uint64_t(row) * bytes};
+    const uint32_t qbox[3] = {uint32_t(128 / bytes), uint32_t(index_score_cols(a->H)), 1};
+    CUtensorMap tk, tq;
+    if (make_tmap(&tk, type, 3, a->index_cache, kdims, kstr, kbox, CU_TENSOR_MAP_SWIZZLE_128B)) return DSA_V32_ERR_DRIVER;
+    if (make_tmap(&tq, type, 3, a->q, qdims, qstr, qbox, CU_TENSOR_MAP_SWIZZLE_128B)) return DSA_V32_ERR_DRIVER;
+    cudaError_t e = launch_index_scores(*a, tk, tq, (cudaStream_t)stream);
     return e == cudaSuccess ? DSA_V32_OK : (int)e;
 }
 
