@@ -950,7 +950,7 @@ int dsa_v32_index_scores(const dsa_v32_index_scores_args* a, void* stream) {
     if (!a) return DSA_V32_ERR_NULL;
     if (a->cache_dtype != DSA_V32_KV_BF16 && a->cache_dtype != DSA_V32_KV_FP8) return DSA_V32_ERR_DTYPE;
     if (a->total_q < 0 || a->s_q <= 0 || a->total_q % a->s_q || a->H <= 0 || a->H > 64 || a->kv_len <= 0) return DSA_V32_ERR_SHAPE;
-    if (a->kv_len > 0x7FFFFFFF - 256) return DSA_V32_ERR_SHAPE;   // positions of a tile behind it stay 32-bit numbers
+    if (a->kv_len > 0x7FFFFFFF - 8192) return DSA_V32_ERR_SHAPE;   // positions of the pages behind it that are looked up stay 32-bit numbers
     if (a->block <= 0 || a->block > 128 || (a->block & (a->block - 1))) return DSA_V32_ERR_SHAPE;
     if (!index_page_ok(a->page_block_size)) return DSA_V32_ERR_SHAPE;
     if (a->num_index_rows <= 0 || a->num_index_rows >= (int64_t(1) << 31) - 1 || a->num_index_rows % a->page_block_size) return DSA_V32_ERR_SHAPE;

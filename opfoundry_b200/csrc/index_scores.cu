@@ -2,14 +2,15 @@
 //
 // The products run on the tensor cores with the positions on the wide side of the tile: D[128 positions][heads of up to 8 query rows] =
 // K Q^T, both operands K-major in shared memory as they lie in global memory (the cache's bytes are never converted).  A TMEM lane is a
-// position, so the sum over heads stays inside a thread, a query row's scores of 32 positions are one 128-byte store, a block's largest
-// one is a few exchanges, and nothing of a NaN or infinite key reaches another position.
+// position, so the sum over heads stays inside a quad of threads, a query row's scores of 32 positions are one 128-byte store, a block's
+// largest one is a few exchanges, and nothing of a NaN or infinite key reaches another position.
 //
 // Roles of a CTA (one an SM): warps 0-15 take the scores out of TMEM (four warpgroups, a query row at a time each), warp 16 brings tiles
 // of 128 keys page by page (TMA; an fp8 cache's scales by bulk copies), warp 17 the query rows, their weights and lengths, warp 18
 // issues the MMAs.  A work item is a group of query rows of one sequence and a chunk of tiles; the CTAs take items in turn, so the
 // ends of short rows (whose columns are only filled) are spread over them.
 #include <cuda_bf16.h>
+#include <cstddef>
 #include <mutex>
 #include "front.h"
 #include "ptx.cuh"
@@ -20,7 +21,7 @@ namespace scores {
 constexpr int kTile = 128;            // positions of a tile: M
 constexpr int kMmaCols = 256;         // most N of an MMA
 constexpr int kTmemCols = 512;
-constexpr int kEpiWarps = 16;
+constexpr int kEpiWarps = 16;          // four warpgroups
 constexpr int kWarps = kEpiWarps + 3;
 constexpr int kMaxRows = 32;          // query rows of a group
 constexpr int kMaxStages = 12;
@@ -50,16 +51,33 @@ struct Params {
     float* out;
     int32_t* status;
     int64_t stride_w_row, stride_o_row, num_pages, seq_stride_pages;
-    int H, s_q, kv_len, limit, block, cols, block_table_stride, page_shift;
+    int H, s_q, kv_len, limit, block, block_shift, cols, block_table_stride, page_shift;
     int per, groups_per_seq, groups;      // query rows of a group, groups of a sequence and of all
     int tiles, chunk, items;
-    int rows_per_acc, acc_cols, slots;    // query rows of an accumulator, its TMEM columns, accumulators in TMEM
+    int acc_cols, slots;                  // narrow: TMEM columns of an accumulator, accumulators in TMEM
     int stages, q_bufs;
     uint32_t off_k, off_s, off_w, q_bytes;   // shared memory: Q buffers | keys | their scales | weights | control
 };
 
 // keys of a stage: bf16 two blocks of 64 columns, fp8 one of 128
 template <bool kFp8> constexpr int kKeyBytes = kFp8 ? kTile * 128 : kTile * 256;
+
+// A warp's wait, bounded: in plain try_waits, whose first usually finds the phase complete, and no sleep in between (with a suspend-time
+// hint a failed try sleeps, and every hand-over in this kernel took some hundred cycles more).  Gives up by time or when another warp has.
+__device__ __forceinline__ bool try_all(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)); }
+__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    const uint64_t t0 = global_ns();
+#pragma unroll 1
+    for (uint32_t n = 1;; ++n) {
+        if (try_all(bar, parity)) return true;
+        if (*abort_flag) return false;
+        if ((n & 63u) == 0 && __any_sync(0xffffffffu, global_ns() - t0 > DSA_WAIT_BUDGET_NS)) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) { return try_all(bar, parity) || wait_on(bar, parity, abort_flag); }
 
 __device__ __forceinline__ float max_nan(float a, float b) {   // NaN where either is
     float d;
@@ -107,6 +125,83 @@ __device__ __forceinline__ Item item_of(const Params& p, int u, int lane) {
     return it;
 }
 
+// ------------------------------------------------ sums over heads
+// 16 lanes x kCols columns of an accumulator: thread t gets, for i < kCols / 8, columns 8 i + 2 (t % 4) and the next of lane t / 4 in
+// d[4 i], d[4 i + 1] and of lane t / 4 + 8 in d[4 i + 2], d[4 i + 3].  So a thread needs the weights of a quarter of the heads only (all of
+// them for every position, read from shared memory for every accumulator, were as many wavefronts as the MMAs' own operands and kept the
+// kernel at 1 800 cycles an accumulator), and the four threads of a quad add up their parts for four positions.
+template <int kCols> __device__ __forceinline__ void load_half(uint32_t taddr, uint32_t (&d)[kCols / 2]) {
+    if constexpr (kCols == 64) {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+            "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7]), "=r"(d[8]), "=r"(d[9]), "=r"(d[10]), "=r"(d[11]),
+              "=r"(d[12]), "=r"(d[13]), "=r"(d[14]), "=r"(d[15]), "=r"(d[16]), "=r"(d[17]), "=r"(d[18]), "=r"(d[19]), "=r"(d[20]), "=r"(d[21]), "=r"(d[22]),
+              "=r"(d[23]), "=r"(d[24]), "=r"(d[25]), "=r"(d[26]), "=r"(d[27]), "=r"(d[28]), "=r"(d[29]), "=r"(d[30]), "=r"(d[31])
+            : "r"(taddr)
+            : "memory");
+    } else if constexpr (kCols == 32) {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7]), "=r"(d[8]), "=r"(d[9]), "=r"(d[10]), "=r"(d[11]),
+              "=r"(d[12]), "=r"(d[13]), "=r"(d[14]), "=r"(d[15])
+            : "r"(taddr)
+            : "memory");
+    } else {
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7])
+                     : "r"(taddr)
+                     : "memory");
+    }
+}
+// where head h's weight stands in its row, so that a thread's are 16 bytes at a time: 16 j + 4 (t % 4) + ..
+__device__ __forceinline__ int weight_at(int h) { return (h & ~15) + 4 * ((h & 7) >> 1) + 2 * ((h >> 3) & 1) + (h & 1); }
+// the position inside the warp's 32 whose sum a thread ends up with
+__device__ __forceinline__ int lane_position(int lane) { return (lane >> 2) + 8 * (lane & 1) + 16 * ((lane >> 1) & 1); }
+// the lane whose position is `off` further on, off a power of two
+__device__ __forceinline__ int lane_of_offset(int off) { return off < 8 ? 4 * off : off >> 3; }
+
+// The sum of w_h max(0, d_h) over a pair of heads is two maxima (half rate) and two multiply-adds.  With max(0, d) taken as (d + |d|) / 2 it is a
+// two-wide multiply-add and two with |d|, three instructions: 533 instead of 540 us for 4096 rows over 16384 positions, and 71.7 instead of 69.1
+// for 64 x 2 rows over 32768, so it stays out.
+struct Sum {
+    float a = 0.0f, b = 0.0f;
+    __device__ __forceinline__ void add(uint32_t d0, uint32_t d1, float u, float v) {
+        a = fmaf(max_nan(__uint_as_float(d0), 0.0f), u, a);
+        b = fmaf(max_nan(__uint_as_float(d1), 0.0f), v, b);
+    }
+    __device__ __forceinline__ float total() const { return a + b; }
+};
+// The row's sum of the thread's position (lane_position).  w: shared-memory address of the thread's first four weights; heads: how many there
+// are, when not all columns are one.
+template <bool kFp8, int kCols, bool kAll>
+__device__ __forceinline__ float sum_heads(const uint32_t (&lo)[kCols / 2], const uint32_t (&hi)[kCols / 2], uint32_t w, int heads, int lane) {
+    Sum s[4];
+#pragma unroll
+    for (int j = 0; j < kCols / 16; ++j) {
+        float w4[4];
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(w4[0]), "=f"(w4[1]), "=f"(w4[2]), "=f"(w4[3]) : "r"(w + 64 * j));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int i = 2 * j + e;
+            uint32_t v[8] = {lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3], hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]};
+            if (!kFp8 && !kAll) {   // columns behind the heads: zeros times an infinite key (e4m3 has none) are NaN
+                const int h = 8 * i + 2 * (lane & 3);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) v[c] = h + (c & 1) < heads ? v[c] : 0u;
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[c].add(v[2 * c], v[2 * c + 1], w4[2 * e], w4[2 * e + 1]);
+        }
+    }
+    // the quad's parts: after the first exchange a thread has two positions, after the second its own
+    const bool b0 = lane & 1, b1 = lane & 2;
+    const float t0 = s[0].total(), t1 = s[1].total(), t2 = s[2].total(), t3 = s[3].total();
+    const float x = (b0 ? t1 : t0) + __shfl_xor_sync(0xffffffffu, b0 ? t0 : t1, 1), y = (b0 ? t3 : t2) + __shfl_xor_sync(0xffffffffu, b0 ? t2 : t3, 1);
+    return (b1 ? y : x) + __shfl_xor_sync(0xffffffffu, b1 ? x : y, 2);
+}
+
 struct Ring {
     int s = 0;
     uint32_t ph = 0;
@@ -116,10 +211,14 @@ struct Ring {
             ph ^= 1u;
         }
     }
+    __device__ __forceinline__ void skip(int by, int n) {
+        for (s += by; s >= n; s -= n) ph ^= 1u;
+    }
 };
 
 // kCols: TMEM columns of a query row, its heads padded to 16, 32 or 64; kAll: there are exactly so many.
-template <bool kFp8, int kCols, bool kAll>
+// kWide: groups of 512 columns.  A tile has two accumulators of 256, and every warpgroup takes its half of one.  Otherwise groups of at most 256 columns, one accumulator a tile, and the warpgroups take tiles in turn.
+template <bool kFp8, int kCols, bool kAll, bool kWide>
 __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tq, const __grid_constant__ Params p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     Control* ctl = reinterpret_cast<Control*>(smem + kSmemBytes - kControlBytes);
@@ -127,31 +226,33 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
     uint8_t* const k_smem = smem + p.off_k;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     volatile int* abort_flag = &ctl->abort_flag;
+    const uint32_t base = smem_u32(smem);
+    auto bar_at = [&](size_t offset, int i) { return base + (uint32_t)(kSmemBytes - kControlBytes + offset) + 8u * i; };
 
     if (tid == 0) {
         for (int i = 0; i < p.stages; ++i) {
-            mbar_init(smem_u32(&ctl->k_full[i]), 1);
-            mbar_init(smem_u32(&ctl->k_empty[i]), 1 + kEpiWarps);
+            mbar_init(bar_at(offsetof(Control, k_full), i), 1);
+            mbar_init(bar_at(offsetof(Control, k_empty), i), 1 + (kWide ? kEpiWarps : 4));
         }
-        for (int i = 0; i < p.slots; ++i) {
-            mbar_init(smem_u32(&ctl->acc_full[i]), 1);
-            mbar_init(smem_u32(&ctl->acc_empty[i]), kEpiWarps);
+        for (int i = 0; i < (kWide ? 2 : p.slots); ++i) {
+            mbar_init(bar_at(offsetof(Control, acc_full), i), 2);
+            mbar_init(bar_at(offsetof(Control, acc_empty), i), kWide ? kEpiWarps / 2 : 4);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&ctl->q_full[i]), 1);
-            mbar_init(smem_u32(&ctl->q_empty[i]), 1);
-            mbar_init(smem_u32(&ctl->w_full[i]), 32);
-            mbar_init(smem_u32(&ctl->w_empty[i]), kEpiWarps);
+            mbar_init(bar_at(offsetof(Control, q_full), i), 1);
+            mbar_init(bar_at(offsetof(Control, q_empty), i), 1);
+            mbar_init(bar_at(offsetof(Control, w_full), i), 32);
+            mbar_init(bar_at(offsetof(Control, w_empty), i), kEpiWarps);
         }
-        for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&ctl->exchange[i]), 4);
+        for (int i = 0; i < 4; ++i) mbar_init(bar_at(offsetof(Control, exchange), i), 4);
         ctl->abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 16 && lane == 0) {
+    if (warp == kEpiWarps && lane == 0) {
         prefetch_tensormap(&tk);
         prefetch_tensormap(&tq);
     }
-    if (warp == 18) {
+    if (warp == kWarps - 1) {
         tmem_alloc(smem_u32(&ctl->tmem_base), kTmemCols);
         tmem_relinquish();
     }
@@ -164,112 +265,125 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
     if (warp < kEpiWarps) {
         // ------------------------------------------------ scores out
         const int wg = warp >> 2, sub = warp & 3;
-        Ring k, slot, wb;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * sub) << 16);
+        const int mine = 32 * sub + lane_position(lane);   // of a tile's positions
+        const int page_bit = mine >> min(p.page_shift, 7), block = p.block, kv_len = p.kv_len;
+        Ring k, acc, wb;
         uint32_t exchanges = 0;
         bool ok = true;
         int u = blockIdx.x;
-        for (; u < p.items && ok; u += gridDim.x) {
-            const Item it = item_of(p, u, lane);
-            if (it.tiles > 0) {
-                ok = warp_wait_short(smem_u32(&ctl->w_full[wb.s]), wb.ph, abort_flag);
-                const float* w = w_smem + wb.s * p.per * kCols;
-                int job = 0;   // (tile, query row) pairs so far: a warpgroup takes every fourth
-                for (int i = 0; i < it.tiles && ok; ++i) {
-                    const int pos = (it.tile0 + i) * kTile + 32 * sub + lane;
-                    float ks = 1.0f;
-                    bool here = false;
-                    for (int r0 = 0; r0 < it.rows; r0 += p.rows_per_acc) {
-                        if (!warp_wait_short(smem_u32(&ctl->acc_full[slot.s]), slot.ph, abort_flag)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        if (r0 == 0) {
-                            if (!warp_wait_short(smem_u32(&ctl->k_full[k.s]), k.ph, abort_flag)) {
-                                ok = false;
-                                break;
-                            }
-                            const uint32_t pages = ctl->page_ok[k.s];
-                            here = (pages >> ((32 * sub + lane) >> min(p.page_shift, 7))) & 1u;
-                            if (kFp8) ks = reinterpret_cast<const float*>(smem + p.off_s + k.s * kScaleBytes)[32 * sub + lane];
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(smem_u32(&ctl->k_empty[k.s]));
-                            k.next(p.stages);
-                        }
-                        const int r1 = min(it.rows, r0 + p.rows_per_acc);
-                        int mine = r0 + ((wg - job) & 3);
-                        const uint32_t acc = tmem + slot.s * p.acc_cols + (static_cast<uint32_t>(32 * sub) << 16);
-                        const uint32_t free_bar = smem_u32(&ctl->acc_empty[slot.s]);
-                        job += r1 - r0;
-                        if (mine >= r1) {   // nothing of this accumulator is this warpgroup's
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(free_bar);
-                        }
-                        for (; mine < r1; mine += 4) {
-                            uint32_t d[kCols];
-                            const uint32_t at = acc + (mine - r0) * kCols;
-                            if constexpr (kCols == 16) {
-                                tmem_ld16(at, d);
-                            } else {
-#pragma unroll
-                                for (int c = 0; c < kCols; c += 32) tmem_ld32(at + c, reinterpret_cast<uint32_t(&)[32]>(d[c]));
-                            }
-                            tmem_wait_ld();
-                            if (mine + 4 >= r1) {
-                                tc_fence_before();
-                                __syncwarp();
-                                if (lane == 0) mbar_arrive(free_bar);
-                            }
-                            const float* wr = w + mine * kCols;
-                            uint64_t s0 = 0, s1 = 0;
-#pragma unroll
-                            for (int h = 0; h < kCols; h += 4) {
-                                const ulonglong2 w2 = *reinterpret_cast<const ulonglong2*>(wr + h);
-                                float v[4];
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    v[j] = max_nan(__uint_as_float(d[h + j]), 0.0f);
-                                    if (!kAll) v[j] = h + j < p.H ? v[j] : 0.0f;   // (zeros times an infinite key)
-                                }
-                                s0 = fma2(pack2(v[0], v[1]), w2.x, s0);
-                                s1 = fma2(pack2(v[2], v[3]), w2.y, s1);
-                            }
-                            float a, b, e, f;
-                            unpack2(s0, a, b);
-                            unpack2(s1, e, f);
-                            float s = ((a + b) + (e + f)) * ks;
-                            s = here && pos < ctl->valid[wb.s][mine] ? s : -INFINITY;
-                            float* out = p.out + (int64_t)(it.q0 + mine) * p.stride_o_row;
-                            if (p.block == 1) {
-                                if (pos < p.kv_len) out[pos] = s;
-                            } else {
-                                for (int off = 1; off < min(p.block, 32); off <<= 1) s = max_nan(s, __shfl_xor_sync(0xffffffffu, s, off));
-                                if (p.block >= 64) {
-                                    const int buf = exchanges & 1;   // (a third job's value is written after the exchange of the second)
-                                    const uint32_t bar = smem_u32(&ctl->exchange[wg]);
-                                    __syncwarp();
-                                    if (lane == 0) {
-                                        ctl->best[wg][buf][sub] = s;
-                                        mbar_arrive(bar);
-                                    }
-                                    ok = ok && warp_wait_short(bar, buf, abort_flag);
-                                    ++exchanges;
-                                    s = max_nan(s, ctl->best[wg][buf][sub ^ 1]);
-                                    if (p.block == 128) s = max_nan(s, max_nan(ctl->best[wg][buf][sub ^ 2], ctl->best[wg][buf][sub ^ 3]));
-                                }
-                                const int col = pos / p.block;
-                                if ((pos & (p.block - 1)) == 0 && col < p.cols) out[col] = s;
-                            }
-                        }
-                        slot.next(p.slots);
-                    }
-                }
+        // A score to its place: s of position pos, -inf unless it counts; `stored`: the row is one.
+        auto put = [&](float s, bool counts, int pos, float* at, bool stored) {
+            s = counts ? s : -INFINITY;
+            if (block == 1) {
+                if (stored && pos < kv_len) *at = s;
+                return;
+            }
+            for (int off = 1; off < min(block, 32); off <<= 1) s = max_nan(s, __shfl_xor_sync(0xffffffffu, s, lane_of_offset(off)));
+            if (block >= 64) {
+                const int buf = exchanges & 1;   // (a third job's value is written after the exchange of the second)
+                const uint32_t bar = bar_at(offsetof(Control, exchange), wg);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&ctl->w_empty[wb.s]));
+                if (lane == 0) {
+                    ctl->best[wg][buf][sub] = s;
+                    mbar_arrive(bar);
+                }
+                ok = ok && wait(bar, buf, abort_flag);
+                ++exchanges;
+                s = max_nan(s, ctl->best[wg][buf][sub ^ 1]);
+                if (block == 128) s = max_nan(s, max_nan(ctl->best[wg][buf][sub ^ 2], ctl->best[wg][buf][sub ^ 3]));
+            }
+            if ((pos & (block - 1)) == 0 && stored && pos < kv_len) *at = s;
+        };
+        // (acc_full has an arrival of the MMA warp's own besides the MMAs': what that warp saw in the tile's barrier is visible here)
+        auto tile_facts = [&](float& ks, bool& here) {
+            here = (ctl->page_ok[k.s] >> page_bit) & 1u;
+            ks = kFp8 ? reinterpret_cast<const float*>(smem + p.off_s + k.s * kScaleBytes)[mine] : 1.0f;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_at(offsetof(Control, k_empty), k.s));
+        };
+        uint32_t lo[kCols / 2], hi[kCols / 2];
+        auto load_row = [&](uint32_t at) {
+            load_half<kCols>(at, lo);
+            load_half<kCols>(at + (16u << 16), hi);
+        };
+        auto give_back = [&](uint32_t bar) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        if constexpr (kWide) {
+            constexpr int kRows = 128 / kCols;                         // of a warpgroup: half of an accumulator
+            const int half = wg >> 1, row0 = wg * kRows;
+            const uint32_t at = lanes + row0 * kCols, full = bar_at(offsetof(Control, acc_full), half), empty = bar_at(offsetof(Control, acc_empty), half);
+            for (; u < p.items && ok; u += gridDim.x) {
+                const Item it = item_of(p, u, lane);
+                if (it.tiles == 0) continue;
+                if (!(ok = wait(bar_at(offsetof(Control, w_full), wb.s), wb.ph, abort_flag))) break;
+                int pos = it.tile0 * kTile + mine, end[kRows];
+                const uint32_t w = base + p.off_w + wb.s * p.per * kCols * 4 + 16 * (lane & 3) + row0 * kCols * 4;
+#pragma unroll
+                for (int j = 0; j < kRows; ++j) end[j] = row0 + j < it.rows ? ctl->valid[wb.s][row0 + j] : -1;   // -1: there is no such row
+                float* out = p.out + (int64_t)(it.q0 + row0) * p.stride_o_row + (pos >> p.block_shift);
+                const int64_t stride = p.stride_o_row;
+                const int step = kTile >> p.block_shift;
+                for (int i = 0; i < it.tiles; ++i, pos += kTile, out += step) {
+                    if (!(ok = ok && wait(full, acc.ph, abort_flag))) break;
+                    tc_fence_after();
+                    load_row(at);
+                    float ks;
+                    bool here;
+                    tile_facts(ks, here);
+                    float* o = out;
+#pragma unroll
+                    for (int j = 0; j < kRows; ++j, o += stride) {
+                        tmem_wait_ld();
+                        if (j == kRows - 1) give_back(empty);
+                        const float s = sum_heads<kFp8, kCols, kAll>(lo, hi, w + j * kCols * 4, p.H, lane) * ks;
+                        if (j + 1 < kRows) load_row(at + (j + 1) * kCols);
+                        put(s, here && pos < end[j], pos, o, end[j] >= 0);
+                    }
+                    acc.ph ^= 1u;
+                    k.next(p.stages);
+                }
+                if (!ok) break;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_at(offsetof(Control, w_empty), wb.s));
                 wb.next(p.q_bufs);
             }
-            if (!ok) break;
+        } else {
+            int turn = wg;                     // tiles until this warpgroup's next one
+            k.skip(wg, p.stages);
+            acc.skip(wg, p.slots);
+            for (; u < p.items && ok; u += gridDim.x) {
+                const Item it = item_of(p, u, lane);
+                if (it.tiles == 0) continue;
+                if (!(ok = wait(bar_at(offsetof(Control, w_full), wb.s), wb.ph, abort_flag))) break;
+                int i = turn;
+                for (; i < it.tiles && ok; i += 4, k.skip(4, p.stages), acc.skip(4, p.slots)) {
+                    const int pos = (it.tile0 + i) * kTile + mine;
+                    if (!(ok = wait(bar_at(offsetof(Control, acc_full), acc.s), acc.ph, abort_flag))) break;
+                    tc_fence_after();
+                    uint32_t at = lanes + acc.s * p.acc_cols, w = base + p.off_w + wb.s * p.per * kCols * 4 + 16 * (lane & 3);
+                    load_row(at);
+                    float ks;
+                    bool here;
+                    tile_facts(ks, here);
+                    float* out = p.out + (int64_t)it.q0 * p.stride_o_row + (pos >> p.block_shift);
+                    for (int r = 0; r < it.rows; ++r, w += kCols * 4, out += p.stride_o_row) {
+                        tmem_wait_ld();
+                        if (r == it.rows - 1) give_back(bar_at(offsetof(Control, acc_empty), acc.s));
+                        const float s = sum_heads<kFp8, kCols, kAll>(lo, hi, w, p.H, lane) * ks;
+                        if (r + 1 < it.rows) load_row(at += kCols);
+                        put(s, here && pos < ctl->valid[wb.s][r], pos, out, true);
+                    }
+                }
+                if (!ok) break;
+                turn = i - it.tiles;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_at(offsetof(Control, w_empty), wb.s));
+                wb.next(p.q_bufs);
+            }
         }
         // The columns behind the last position that a row of an item sees, once nothing waits for this warp any more.  After a wait that
         // gave up: all of the items that were not finished.
@@ -282,25 +396,37 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
                 for (int c = c0 + (lost ? lane : tid); c < c1; c += lost ? 32 : 32 * kEpiWarps)
                     p.out[(int64_t)(it.q0 + r) * p.stride_o_row + c] = lost ? __int_as_float(0x7FFFFFFF) : -INFINITY;
         }
-    } else if (warp == 16) {
+    } else if (warp == kEpiWarps) {
         // ------------------------------------------------ keys in
         Ring k;
         const int page_rows = 1 << min(p.page_shift, 7), pages = kTile / page_rows;   // of a tile
         bool ok = true;
         for (int u = blockIdx.x; u < p.items && ok; u += gridDim.x) {
             const Item it = item_of(p, u, lane);
-            for (int i = 0; i < it.tiles; ++i, k.next(p.stages)) {
-                const int pos = (it.tile0 + i) * kTile;
+            // Page numbers come 32 at a time, a batch ahead of their use (a load of them per tile was 700 clocks of every tile).
+            const int per_batch = 32 / pages;   // tiles of a batch
+            auto batch = [&](int first) {
+                const int pos = (it.tile0 + first) * kTile + lane * page_rows;
                 int64_t page = -1;
-                if (lane < pages) {
-                    const int blk = (pos >> p.page_shift) + lane;
+                if (first < it.tiles) {
+                    const int blk = pos >> p.page_shift;
                     if (p.block_table == nullptr) page = (int64_t)it.seq * p.seq_stride_pages + blk;
                     else if (blk < p.block_table_stride) page = __ldg(p.block_table + (int64_t)it.seq * p.block_table_stride + blk);
-                    if (page < 0 || page >= p.num_pages) page = -1;
                 }
+                return page >= 0 && page < p.num_pages ? (int)page : -1;
+            };
+            int now = -1, ahead = batch(0);
+            for (int i = 0; i < it.tiles; ++i, k.next(p.stages)) {
+                const int pos = (it.tile0 + i) * kTile, in_batch = i & (per_batch - 1);
+                if (in_batch == 0) {
+                    now = ahead;
+                    ahead = batch(i + per_batch);
+                }
+                const int got = __shfl_sync(0xffffffffu, now, (in_batch * pages + lane) & 31);
+                const int64_t page = lane < pages ? got : -1;
                 const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
-                if (!(ok = warp_wait(smem_u32(&ctl->k_empty[k.s]), k.ph ^ 1u, abort_flag))) break;
-                const uint32_t bar = smem_u32(&ctl->k_full[k.s]), dst = smem_u32(k_smem + k.s * kKeyBytes<kFp8>);
+                if (!(ok = wait(bar_at(offsetof(Control, k_empty), k.s), k.ph ^ 1u, abort_flag))) break;
+                const uint32_t bar = bar_at(offsetof(Control, k_full), k.s), dst = smem_u32(k_smem + k.s * kKeyBytes<kFp8>);
                 if (lane == 0) {
                     ctl->page_ok[k.s] = there;
                     mbar_arrive_expect_tx(bar, kKeyBytes<kFp8> + (kFp8 ? __popc(there) * page_rows * 4 : 0));
@@ -317,34 +443,34 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
                 }
             }
         }
-    } else if (warp == 17) {
+    } else if (warp == kEpiWarps + 1) {
         // ------------------------------------------------ query rows, weights, lengths in
         Ring b;
         bool ok = true;
         for (int u = blockIdx.x; u < p.items && ok; u += gridDim.x) {
             const Item it = item_of(p, u, lane);
             if (it.tiles == 0) continue;
-            if (!(ok = warp_wait(smem_u32(&ctl->q_empty[b.s]), b.ph ^ 1u, abort_flag))) break;
-            const uint32_t bar = smem_u32(&ctl->q_full[b.s]), dst = smem_u32(smem) + b.s * p.q_bytes;
+            if (!(ok = wait(bar_at(offsetof(Control, q_empty), b.s), b.ph ^ 1u, abort_flag))) break;
+            const uint32_t bar = bar_at(offsetof(Control, q_full), b.s), dst = smem_u32(smem) + b.s * p.q_bytes;
             if (lane == 0) mbar_arrive_expect_tx(bar, it.rows * kCols * (kFp8 ? 128 : 256));
             __syncwarp();
             if (lane < it.rows) {
                 tma_load_3d(dst + lane * kCols * 128, &tq, bar, 0, 0, it.q0 + lane);
                 if (!kFp8) tma_load_3d(dst + p.q_bytes / 2 + lane * kCols * 128, &tq, bar, 64, 0, it.q0 + lane);
             }
-            if (!(ok = warp_wait(smem_u32(&ctl->w_empty[b.s]), b.ph ^ 1u, abort_flag))) break;
+            if (!(ok = wait(bar_at(offsetof(Control, w_empty), b.s), b.ph ^ 1u, abort_flag))) break;
             float* w = w_smem + b.s * p.per * kCols;
             for (int i = lane; i < it.rows * kCols; i += 32) {
                 const int r = i / kCols, h = i % kCols;
-                w[i] = h < p.H ? __ldg(p.weights + (int64_t)(it.q0 + r) * p.stride_w_row + h) : 0.0f;
+                w[r * kCols + weight_at(h)] = h < p.H ? __ldg(p.weights + (int64_t)(it.q0 + r) * p.stride_w_row + h) : 0.0f;
             }
             if (lane < it.rows) ctl->valid[b.s][lane] = row_limit(p, it.q0 + lane);
-            mbar_arrive(smem_u32(&ctl->w_full[b.s]));
+            mbar_arrive(bar_at(offsetof(Control, w_full), b.s));
             b.next(p.q_bufs);
         }
     } else {
         // ------------------------------------------------ MMAs
-        Ring k, slot, b;
+        Ring k, acc, b;
         bool ok = true;
         const uint32_t el = elect_one() ? 1u : 0u;
         const uint64_t k_desc = make_smem_desc_sw128(smem_u32(k_smem), 0, 1024), q_desc = make_smem_desc_sw128(smem_u32(smem), 0, 1024);
@@ -352,27 +478,31 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
         for (int u = blockIdx.x; u < p.items && ok; u += gridDim.x) {
             const Item it = item_of(p, u, lane);
             if (it.tiles == 0) continue;
-            if (!(ok = warp_wait(smem_u32(&ctl->q_full[b.s]), b.ph, abort_flag))) break;
+            if (!(ok = wait(bar_at(offsetof(Control, q_full), b.s), b.ph, abort_flag))) break;
             for (int i = 0; i < it.tiles && ok; ++i, k.next(p.stages)) {
-                if (!(ok = warp_wait(smem_u32(&ctl->k_full[k.s]), k.ph, abort_flag))) break;
-                for (int r0 = 0; r0 < it.rows; r0 += p.rows_per_acc, slot.next(p.slots)) {
-                    if (!(ok = warp_wait(smem_u32(&ctl->acc_empty[slot.s]), slot.ph ^ 1u, abort_flag))) break;
+                if (!(ok = wait(bar_at(offsetof(Control, k_full), k.s), k.ph, abort_flag))) break;
+#pragma unroll
+                for (int part = 0; part < (kWide ? 2 : 1); ++part) {
+                    if (!(ok = ok && wait(bar_at(offsetof(Control, acc_empty), acc.s), acc.ph ^ 1u, abort_flag))) break;
                     tc_fence_after();
-                    const int n = min(p.rows_per_acc, it.rows - r0) * kCols;
-                    const uint32_t a = k_lo + ((k.s * kKeyBytes<kFp8>) >> 4), q = q_lo + ((b.s * p.q_bytes + r0 * kCols * 128) >> 4), acc = tmem + slot.s * p.acc_cols;
+                    const int n = kWide ? kMmaCols : it.rows * kCols;   // (wide: rows that there are not are never read back)
+                    const uint32_t a = k_lo + ((k.s * kKeyBytes<kFp8>) >> 4), q = q_lo + ((b.s * p.q_bytes + part * kMmaCols * 128) >> 4);
+                    const uint32_t d = tmem + acc.s * (kWide ? kMmaCols : p.acc_cols), full = bar_at(offsetof(Control, acc_full), acc.s);
                     if constexpr (kFp8) {
-                        umma_f8_ss_x4_el(acc, a, hi, q, hi, make_idesc_e4m3(kTile, n), el);
+                        umma_f8_ss_x4_el(d, a, hi, q, hi, make_idesc_e4m3(kTile, n), el);
                     } else {
                         const uint32_t idesc = make_idesc_bf16(kTile, n, false);
-                        umma_ss_x4_el(acc, a, hi, q, hi, idesc, 0u, el);
-                        umma_ss_x4_el(acc, a + ((kTile * 128) >> 4), hi, q + ((p.q_bytes / 2) >> 4), hi, idesc, 1u, el);
+                        umma_ss_x4_el(d, a, hi, q, hi, idesc, 0u, el);
+                        umma_ss_x4_el(d, a + ((kTile * 128) >> 4), hi, q + ((p.q_bytes / 2) >> 4), hi, idesc, 1u, el);
                     }
-                    tc_commit_el(smem_u32(&ctl->acc_full[slot.s]), el);
+                    tc_commit_el(full, el);
+                    if (el) mbar_arrive(full);
+                    acc.next(kWide ? 2 : p.slots);
                 }
-                if (ok) tc_commit_el(smem_u32(&ctl->k_empty[k.s]), el);
+                if (ok) tc_commit_el(bar_at(offsetof(Control, k_empty), k.s), el);
             }
             if (!ok) break;
-            tc_commit_el(smem_u32(&ctl->q_empty[b.s]), el);
+            tc_commit_el(bar_at(offsetof(Control, q_empty), b.s), el);
             b.next(p.q_bufs);
         }
     }
@@ -384,13 +514,13 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
         settle_in_flight();
         __syncthreads();
     }
-    if (warp == 18) {
+    if (warp == kWarps - 1) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
     }
 }
 
-template <bool kFp8, int kCols, bool kAll>
+template <bool kFp8, int kCols, bool kAll, bool kWide>
 cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tq, const Params& p, int grid, cudaStream_t stream) {
     static std::mutex mu;
     static bool done[64] = {};
@@ -400,7 +530,7 @@ cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tq, const Params& p
     {
         std::lock_guard<std::mutex> guard(mu);
         if (dev < 0 || dev >= 64 || !done[dev]) {
-            e = cudaFuncSetAttribute(index_scores_kernel<kFp8, kCols, kAll>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+            e = cudaFuncSetAttribute(index_scores_kernel<kFp8, kCols, kAll, kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
             if (e != cudaSuccess) return e;
             if (dev >= 0 && dev < 64) done[dev] = true;
         }
@@ -415,7 +545,7 @@ cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tq, const Params& p
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, index_scores_kernel<kFp8, kCols, kAll>, tk, tq, p);
+    return cudaLaunchKernelEx(&cfg, index_scores_kernel<kFp8, kCols, kAll, kWide>, tk, tq, p);
 }
 
 }  // namespace scores
@@ -447,18 +577,23 @@ cudaError_t launch_index_scores(const dsa_v32_index_scores_args& a, const CUtens
     const int64_t reach = a.block_table ? (int64_t)a.block_table_stride << p.page_shift : a.kv_batch_stride_rows;
     if (reach > 0 && reach < p.limit) p.limit = (int)reach;
     p.block = a.block;
+    while ((1 << p.block_shift) < a.block) ++p.block_shift;
     p.cols = (a.kv_len + a.block - 1) / a.block;
     p.block_table_stride = a.block_table_stride;
-    // query rows of a group: as many as TMEM has columns for, in groups of equal size
+    // Query rows of a group: 512 columns' worth where a sequence fills most of them, else up to 256 in groups of equal size (a group of
+    // 512 reads the keys half as often, but takes two full accumulators of every tile however many rows there are).
     const int most = kTmemCols / cols;
-    p.groups_per_seq = (a.s_q + most - 1) / most;
-    p.per = (a.s_q + p.groups_per_seq - 1) / p.groups_per_seq;
+    const bool wide = 4 * a.s_q >= 3 * most;
+    p.per = most;
+    if (!wide) {
+        const int n = (a.s_q + most / 2 - 1) / (most / 2);
+        p.per = (a.s_q + n - 1) / n;
+    }
     p.groups_per_seq = (a.s_q + p.per - 1) / p.per;
     const int64_t groups = (int64_t)p.groups_per_seq * (a.total_q / a.s_q);
-    const int accs = (p.per * cols + kMmaCols - 1) / kMmaCols;
-    p.rows_per_acc = (p.per + accs - 1) / accs;
-    p.acc_cols = (p.rows_per_acc * cols + 31) & ~31;
-    p.slots = kTmemCols / p.acc_cols < kMaxSlots ? kTmemCols / p.acc_cols : kMaxSlots;
+    p.acc_cols = 64;
+    while (p.acc_cols < p.per * cols) p.acc_cols *= 2;
+    p.slots = wide ? 2 : kTmemCols / p.acc_cols;
     // shared memory: two buffers of query rows where that leaves four stages of keys
     const int stage = fp8 ? kKeyBytes<true> + kScaleBytes : kKeyBytes<false>;
     p.q_bytes = p.per * cols * (fp8 ? 128 : 256);
@@ -486,14 +621,19 @@ cudaError_t launch_index_scores(const dsa_v32_index_scores_args& a, const CUtens
     const int grid = (int)(items < sms ? items : sms);
     const bool all = a.H == cols;
     auto go = [&](auto kernel) { return kernel(tk, tq, p, grid, stream); };
-    if (fp8) {
-        if (cols == 16) return go(all ? launch<true, 16, true> : launch<true, 16, false>);
-        if (cols == 32) return go(all ? launch<true, 32, true> : launch<true, 32, false>);
-        return go(all ? launch<true, 64, true> : launch<true, 64, false>);
+#define DSA_SCORES_OF(fp8_, cols_)                                                                                       \
+    if (fp8 == fp8_ && cols == cols_) {                                                                                  \
+        if (wide) return go(all ? launch<fp8_, cols_, true, true> : launch<fp8_, cols_, false, true>);                   \
+        return go(all ? launch<fp8_, cols_, true, false> : launch<fp8_, cols_, false, false>);                           \
     }
-    if (cols == 16) return go(all ? launch<false, 16, true> : launch<false, 16, false>);
-    if (cols == 32) return go(all ? launch<false, 32, true> : launch<false, 32, false>);
-    return go(all ? launch<false, 64, true> : launch<false, 64, false>);
+    DSA_SCORES_OF(true, 16)
+    DSA_SCORES_OF(true, 32)
+    DSA_SCORES_OF(true, 64)
+    DSA_SCORES_OF(false, 16)
+    DSA_SCORES_OF(false, 32)
+    DSA_SCORES_OF(false, 64)
+#undef DSA_SCORES_OF
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace dsa
