@@ -7,6 +7,7 @@ happens in the CUDA library, and importing this module without the built library
 """
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -139,9 +140,8 @@ def lib():
         L.dsa_v32_debug_rows.argtypes = [C.POINTER(AttnArgs), C.c_void_p, C.c_void_p]
         L.dsa_v32_topk_select.argtypes = [C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]
         L.dsa_v32_pack_fp8_rows.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
-        L.dsa_v32_norm_rotate.argtypes = [C.POINTER(NormRotateArgs), C.c_void_p]
-        L.dsa_v32_append_cache.argtypes = [C.POINTER(AppendArgs), C.c_void_p]
-        L.dsa_v32_index_scores.argtypes = [C.POINTER(IndexScoresArgs), C.c_void_p]
+        for name in ("dsa_v32_norm_rotate", "dsa_v32_append_cache", "dsa_v32_index_scores"):
+            getattr(L, name).argtypes = [C.c_void_p, C.c_void_p]   # a structure by reference, or its bytes
         L.dsa_v32_block_select.argtypes = [C.c_void_p, C.c_int64, C.c_void_p] + [C.c_int32] * 6 + [C.c_void_p, C.c_void_p]
         _lib = L
     return _lib
@@ -405,21 +405,29 @@ def mla_decode_launch_pipeline_static(q, kv, indices, sm_scale, *, s_q=1, block_
 # ------------------------------------------------------------------ the front end: from a layer's projections to the attention's lists
 DTYPE_BF16, DTYPE_FP32, DTYPE_E4M3 = 0, 1, 2
 _IN_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_FP32}
-_OUT_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float8_e4m3fn: DTYPE_E4M3}
+
+
+# The argument blocks as bytes: packing one takes a fraction of the time of a ctypes structure with forty fields (append_cache 12.3 -> 7.5 us of host
+# time a call with the checks below written flat).
+_NORM_ROTATE, _APPEND, _INDEX_SCORES = struct.Struct("@13Q8q11if"), struct.Struct("@12Q5q11if"), struct.Struct("@7Q6q8i")
+_BF16, _F32, _I32, _U8, _E4M3 = torch.bfloat16, torch.float32, torch.int32, torch.uint8, torch.float8_e4m3fn
 
 
 def _here(*tensors):
     """All tensors live on the current device: the launch goes to its current stream."""
     dev = torch._C._cuda_getDevice()
     for t in tensors:
-        assert t is None or t.get_device() == dev, "a tensor is not on the current device"
+        if t is not None and t.get_device() != dev:
+            raise AssertionError("a tensor is not on the current device")
+    return dev
 
 
-def _vec(t, n, dtype=torch.float32):
-    """Address of a dense vector of n values, or None."""
+def _vec(t, n, dtype=_F32):
+    """Address of a dense vector of n values, 0 for None."""
     if t is None:
-        return None
-    assert t.dtype == dtype and t.numel() == n and t.is_contiguous()
+        return 0
+    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
+        raise AssertionError("expected %d dense values of %s" % (n, dtype))
     return t.data_ptr()
 
 
@@ -432,44 +440,45 @@ def norm_rotate(q, cos_sin, positions, *, k=None, q_weight=None, k_weight=None, 
     on are rotated in pairs (2 i, 2 i + 1), or (i, i + rope_dim / 2) when not `interleaved`.  positions int32 [tokens]: nothing is written for
     one outside the table (padding).  e4m3 out: each head's values over its scale amax / 448; q's scales are multiplied by
     head_weight [tokens, heads].  q_out may be q.  Returns (q_out, k_out, q_scale, k_scale), None where there is none."""
-    if q_out is not None:
-        out_dtype = q_out.dtype
-    T, H, D = q.shape
-    assert q.dtype in _IN_DTYPES and out_dtype in _OUT_DTYPES and (D == 1 or q.stride(2) == 1)
-    e4m3 = out_dtype == torch.float8_e4m3fn
-    Hk = 0
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+    T, H, D = shape = q.shape
+    (qs0, qs1, qs2), (qo0, qo1, qo2) = q.stride(), q_out.stride()
+    out_dtype = q_out.dtype
+    e4m3 = out_dtype is _E4M3
+    assert q.dtype in _IN_DTYPES and (e4m3 or out_dtype is _BF16) and q_out.shape == shape and qs2 == 1 and qo2 == 1
+    Hk = ks0 = ks1 = ko0 = ko1 = k_at = k_out_at = 0
     if k is not None:
         Hk = k.shape[1]
-        assert k.dtype == q.dtype and k.shape == (T, Hk, D) and Hk > 0 and k.stride(2) == 1
         if k_out is None:
-            k_out = torch.empty(T, Hk, D, dtype=out_dtype, device=q.device)
-        assert k_out.dtype == out_dtype and k_out.shape == k.shape and k_out.stride(2) == 1
+            k_out = torch.empty(k.shape, dtype=out_dtype, device=q.device)
+        (ks0, ks1, ks2), (ko0, ko1, ko2) = k.stride(), k_out.stride()
+        assert k.dtype is q.dtype and k.shape == (T, Hk, D) and Hk > 0 and k_out.dtype is out_dtype and k_out.shape == k.shape and ks2 == 1 and ko2 == 1
+        k_at, k_out_at = k.data_ptr(), k_out.data_ptr()
     else:
         assert k_out is None and k_weight is None and k_bias is None and k_scale is None
-    if q_out is None:
-        q_out = torch.empty(T, H, D, dtype=out_dtype, device=q.device)
-    assert q_out.shape == q.shape and q_out.stride(2) == 1
     if e4m3:
         if q_scale is None:
-            q_scale = torch.empty(T, H, dtype=torch.float32, device=q.device)
+            q_scale = torch.empty(T, H, dtype=_F32, device=q.device)
         if Hk and k_scale is None:
-            k_scale = torch.empty(T, Hk, dtype=torch.float32, device=q.device)
+            k_scale = torch.empty(T, Hk, dtype=_F32, device=q.device)
     else:
         assert q_scale is None and k_scale is None and head_weight is None
-    _here(q, k, q_out, k_out, q_scale, k_scale, q_weight, q_bias, k_weight, k_bias, head_weight, cos_sin, positions)
-    R = P = 0
+    dev = _here(q, q_out, k, k_out, q_scale, k_scale, q_weight, q_bias, k_weight, k_bias, head_weight, cos_sin, positions)
+    R = P = table = 0
     if cos_sin is not None:
-        assert cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.is_contiguous() and positions is not None
         P, R = cos_sin.shape
+        assert cos_sin.dtype is _F32 and cos_sin.is_contiguous() and positions is not None
+        table = cos_sin.data_ptr()
     elif positions is not None:
         P = 0x7FFFFFFF      # no table: every position from 0 on
-    qs, qo = q.stride(), q_out.stride()
-    ks, ko = (k.stride(), k_out.stride()) if Hk else ((0, 0), (0, 0))
-    a = NormRotateArgs(q.data_ptr(), k.data_ptr() if Hk else None, q_out.data_ptr(), k_out.data_ptr() if Hk else None, _vec(q_scale, T * H),
-                       _vec(k_scale, T * Hk), _vec(q_weight, D), _vec(q_bias, D), _vec(k_weight, D), _vec(k_bias, D), _vec(head_weight, T * H),
-                       cos_sin.data_ptr() if R else None, _vec(positions, T, torch.int32), qs[0], qs[1], ks[0], ks[1], qo[0], qo[1], ko[0], ko[1],
-                       T, H, Hk, D, rope_begin, R, P, _IN_DTYPES[q.dtype], _OUT_DTYPES[out_dtype], 1 if interleaved else 0, 1 if center else 0, eps)
-    _check(lib().dsa_v32_norm_rotate(C.byref(a), _stream()), "dsa_v32_norm_rotate")
+    a = _NORM_ROTATE.pack(q.data_ptr(), k_at, q_out.data_ptr(), k_out_at, _vec(q_scale, T * H), _vec(k_scale, T * Hk), _vec(q_weight, D), _vec(q_bias, D),
+                          _vec(k_weight, D), _vec(k_bias, D), _vec(head_weight, T * H), table, _vec(positions, T, _I32), qs0, qs1, ks0, ks1, qo0, qo1,
+                          ko0, ko1, T, H, Hk, D, rope_begin, R, P, _IN_DTYPES[q.dtype], DTYPE_E4M3 if e4m3 else DTYPE_BF16, 1 if interleaved else 0,
+                          1 if center else 0, eps)
+    status = lib().dsa_v32_norm_rotate(a, torch._C._cuda_getCurrentRawStream(dev))
+    if status:
+        raise DsaError(status, "dsa_v32_norm_rotate")
     return q_out, k_out, q_scale, k_scale
 
 
@@ -482,19 +491,24 @@ def index_cache_pages(num_pages, fp8, page_block_size=64, device="cuda"):
 
 def _index_rows(cache, page_block_size):
     """(type, rows) of an index cache."""
-    assert cache.is_contiguous() and cache.dim() == 2
-    if cache.dtype == torch.uint8:
-        assert cache.shape[1] == page_block_size * (D_INDEX + 4)
-        return KV_FP8, cache.shape[0] * page_block_size
-    assert cache.dtype == torch.bfloat16 and cache.shape[1] == D_INDEX
-    return KV_BF16, cache.shape[0]
+    n, width = cache.shape
+    if not cache.is_contiguous():
+        raise AssertionError("the index cache is not dense")
+    if cache.dtype is _U8 and width == page_block_size * (D_INDEX + 4):
+        return KV_FP8, n * page_block_size
+    if cache.dtype is _BF16 and width == D_INDEX:
+        return KV_BF16, n
+    raise AssertionError("an index cache is uint8 [pages, page * 132] or bf16 [pages * page, 128]")
 
 
 def _table(block_table):
+    """(address, sequences, pages of a sequence)."""
     if block_table is None:
-        return None, 0, 0
-    assert block_table.dtype == torch.int32 and block_table.is_contiguous() and block_table.dim() == 2
-    return block_table.data_ptr(), block_table.shape[0], block_table.shape[1]
+        return 0, 0, 0
+    n, width = block_table.shape
+    if block_table.dtype is not _I32 or not block_table.is_contiguous():
+        raise AssertionError("the block table is dense int32")
+    return block_table.data_ptr(), n, width
 
 
 def append_cache(latent, rope, kv, cos_sin, positions, *, seq_ids=None, s_q=1, block_table=None, page_block_size=64, kv_batch_stride_rows=0,
@@ -506,33 +520,45 @@ def append_cache(latent, rope, kv, cos_sin, positions, *, seq_ids=None, s_q=1, b
     seq_ids[t] (None: t // s_q); a negative sequence, a position outside cos_sin [positions, 64] or a row outside the cache writes nothing.
     latent = rope = kv = None: the index cache alone."""
     tokens = positions.shape[0]
-    x = latent if latent is not None else index_key
-    assert x is not None and x.dtype in _IN_DTYPES
-    assert cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.shape[1] == D_ROPE and cos_sin.is_contiguous()
-    _here(latent, rope, kv, cos_sin, positions, seq_ids, block_table, latent_weight, index_key, index_cache, index_weight, index_bias)
-    kinds = []
+    P, R = cos_sin.shape
+    assert cos_sin.dtype is _F32 and R == D_ROPE and cos_sin.is_contiguous()
+    dev = _here(latent, rope, kv, cos_sin, positions, seq_ids, block_table, latent_weight, index_key, index_cache, index_weight, index_bias)
+    latent_at = rope_at = kv_at = key_at = cache_at = latent_stride = rope_stride = key_stride = 0
+    dtype = kind = None
     if kv is not None:
-        assert latent.shape == (tokens, D_V) and rope.shape == (tokens, D_ROPE) and rope.dtype == x.dtype and latent.stride(1) == 1 and rope.stride(1) == 1
-        assert kv.is_contiguous() and (kv.dtype, kv.shape[-1]) in ((torch.uint8, FP8_ROW_BYTES), (torch.bfloat16, D_QK))
-        kinds.append((KV_FP8 if kv.dtype == torch.uint8 else KV_BF16, kv.numel() // kv.shape[-1]))
+        dtype, width = latent.dtype, kv.shape[-1]
+        (latent_stride, l1), (rope_stride, r1) = latent.stride(), rope.stride()
+        assert latent.shape == (tokens, D_V) and rope.shape == (tokens, D_ROPE) and rope.dtype is dtype and l1 == 1 and r1 == 1 and kv.is_contiguous()
+        if kv.dtype is _U8:
+            kind = KV_FP8
+            assert width == FP8_ROW_BYTES
+        else:
+            kind = KV_BF16
+            assert kv.dtype is _BF16 and width == D_QK
+        rows = kv.numel() // width
+        latent_at, rope_at, kv_at = latent.data_ptr(), rope.data_ptr(), kv.data_ptr()
     else:
-        assert latent is None and rope is None and latent_weight is None
+        assert latent is None and rope is None and latent_weight is None and index_cache is not None
     if index_cache is not None:
-        assert index_key.shape == (tokens, D_INDEX) and index_key.dtype == x.dtype and index_key.stride(1) == 1
-        kinds.append(_index_rows(index_cache, page_block_size))
+        index_kind, index_rows = _index_rows(index_cache, page_block_size)
+        key_stride, k1 = index_key.stride()
+        assert index_key.shape == (tokens, D_INDEX) and k1 == 1
+        if kv is None:
+            dtype, kind, rows = index_key.dtype, index_kind, index_rows
+        assert index_key.dtype is dtype and index_kind == kind and index_rows == rows, "the two caches have different types or rows"
+        key_at, cache_at = index_key.data_ptr(), index_cache.data_ptr()
     else:
         assert index_key is None and index_weight is None and index_bias is None
-    assert len(kinds) == 1 or kinds[0] == kinds[1], "the two caches have different types or rows"
     table, num_seqs, table_stride = _table(block_table)
-    a = AppendArgs(latent.data_ptr() if kv is not None else None, rope.data_ptr() if kv is not None else None,
-                   index_key.data_ptr() if index_cache is not None else None, kv.data_ptr() if kv is not None else None,
-                   index_cache.data_ptr() if index_cache is not None else None, _vec(latent_weight, D_V), _vec(index_weight, D_INDEX),
-                   _vec(index_bias, D_INDEX), cos_sin.data_ptr(), _vec(positions, tokens, torch.int32), _vec(seq_ids, tokens, torch.int32), table,
-                   latent.stride(0) if kv is not None else 0, rope.stride(0) if kv is not None else 0,
-                   index_key.stride(0) if index_cache is not None else 0, kinds[0][1], kv_batch_stride_rows, tokens, s_q, num_seqs, table_stride,
-                   page_block_size, cos_sin.shape[0], _IN_DTYPES[x.dtype], kinds[0][0], 1 if interleaved else 0,
-                   1 if (interleaved if index_interleaved is None else index_interleaved) else 0, 1 if index_center else 0, eps)
-    _check(lib().dsa_v32_append_cache(C.byref(a), _stream()), "dsa_v32_append_cache")
+    if index_interleaved is None:
+        index_interleaved = interleaved
+    a = _APPEND.pack(latent_at, rope_at, key_at, kv_at, cache_at, _vec(latent_weight, D_V), _vec(index_weight, D_INDEX), _vec(index_bias, D_INDEX),
+                     cos_sin.data_ptr(), _vec(positions, tokens, _I32), _vec(seq_ids, tokens, _I32), table, latent_stride, rope_stride, key_stride, rows,
+                     kv_batch_stride_rows, tokens, s_q, num_seqs, table_stride, page_block_size, P, _IN_DTYPES[dtype], kind, 1 if interleaved else 0,
+                     1 if index_interleaved else 0, 1 if index_center else 0, eps)
+    status = lib().dsa_v32_append_cache(a, torch._C._cuda_getCurrentRawStream(dev))
+    if status:
+        raise DsaError(status, "dsa_v32_append_cache")
 
 
 def index_scores(q, weights, index_cache, valid_len, kv_len, *, s_q=1, block=1, block_table=None, page_block_size=64, kv_batch_stride_rows=0, out=None,
@@ -545,31 +571,39 @@ def index_scores(q, weights, index_cache, valid_len, kv_len, *, s_q=1, block=1, 
     status: int32 [1], gets ERR_DEVICE_WAIT where a bounded wait in the kernel ran out (the scores are then NaN)."""
     total_q, H, D = q.shape
     kind, rows = _index_rows(index_cache, page_block_size)
-    assert D == D_INDEX and q.stride(2) == 1 and q.dtype == (torch.float8_e4m3fn if kind == KV_FP8 else torch.bfloat16)
-    assert weights.dtype == torch.float32 and weights.shape == (total_q, H) and (H == 1 or weights.stride(1) == 1)
+    q0, q1, q2 = q.stride()
+    w0, w1 = weights.stride()
     cols = -(-kv_len // block)
     if out is None:
-        out = torch.empty(total_q, cols, dtype=torch.float32, device=q.device)
-    assert out.dtype == torch.float32 and out.shape == (total_q, cols) and (cols == 1 or out.stride(1) == 1)
-    _here(q, weights, index_cache, valid_len, block_table, out, status)
+        out = torch.empty(total_q, cols, dtype=_F32, device=q.device)
+    o0, o1 = out.stride()
+    assert D == D_INDEX and q2 == 1 and q.dtype is (_E4M3 if kind == KV_FP8 else _BF16)
+    assert weights.dtype is _F32 and weights.shape == (total_q, H) and (H == 1 or w1 == 1)
+    assert out.dtype is _F32 and out.shape == (total_q, cols) and (cols == 1 or o1 == 1)
+    dev = _here(q, weights, index_cache, valid_len, block_table, out, status)
     table, num_seqs, table_stride = _table(block_table)
-    assert table is None or num_seqs * s_q >= total_q, "the block table has fewer rows than there are sequences"
-    a = IndexScoresArgs(q.data_ptr(), weights.data_ptr(), index_cache.data_ptr(), _vec(valid_len, total_q, torch.int32), table, out.data_ptr(),
-                        _vec(status, 1, torch.int32), q.stride(0), q.stride(1), weights.stride(0), out.stride(0), rows, kv_batch_stride_rows,
-                        total_q, H, s_q, kv_len, block, table_stride, page_block_size, kind)
-    _check(lib().dsa_v32_index_scores(C.byref(a), _stream()), "dsa_v32_index_scores")
+    assert not table or num_seqs * s_q >= total_q, "the block table has fewer rows than there are sequences"
+    a = _INDEX_SCORES.pack(q.data_ptr(), weights.data_ptr(), index_cache.data_ptr(), _vec(valid_len, total_q, _I32), table, out.data_ptr(),
+                           _vec(status, 1, _I32), q0, q1, w0, o0, rows, kv_batch_stride_rows, total_q, H, s_q, kv_len, block, table_stride,
+                           page_block_size, kind)
+    rc = lib().dsa_v32_index_scores(a, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        raise DsaError(rc, "dsa_v32_index_scores")
     return out
 
 
 def block_select(scores, num_selected, block, valid_len=None, *, first=0, local=0, out=None):
     """scores fp32 [rows, blocks] (index_scores) -> int32 [rows, num_selected * block]: the positions below valid_len [rows] (None: all) of
     the num_selected best blocks of every row, the first `first` and last `local` ones always among them; ascending, -1 padded."""
-    assert scores.dtype == torch.float32 and scores.dim() == 2 and (scores.shape[1] == 1 or scores.stride(1) == 1)
     rows, blocks = scores.shape
+    s0, s1 = scores.stride()
     if out is None:
-        out = torch.empty(rows, num_selected * block, dtype=torch.int32, device=scores.device)
-    assert out.dtype == torch.int32 and out.shape == (rows, num_selected * block) and out.is_contiguous()
-    _here(scores, valid_len, out)
-    _check(lib().dsa_v32_block_select(scores.data_ptr(), scores.stride(0) if rows > 1 else blocks, _vec(valid_len, rows, torch.int32), rows, blocks, block,
-                                      num_selected, first, local, out.data_ptr(), _stream()), "dsa_v32_block_select")
+        out = torch.empty(rows, num_selected * block, dtype=_I32, device=scores.device)
+    assert scores.dtype is _F32 and (blocks == 1 or s1 == 1)
+    assert out.dtype is _I32 and out.shape == (rows, num_selected * block) and out.is_contiguous()
+    dev = _here(scores, valid_len, out)
+    status = lib().dsa_v32_block_select(scores.data_ptr(), s0 if rows > 1 else blocks, _vec(valid_len, rows, _I32), rows, blocks, block, num_selected, first,
+                                        local, out.data_ptr(), torch._C._cuda_getCurrentRawStream(dev))
+    if status:
+        raise DsaError(status, "dsa_v32_block_select")
     return out
