@@ -4,6 +4,7 @@
 // pairs of its rotated values turned by the angle of the token's position, then one rounding to bf16, or to e4m3 with scale = amax / 448.
 // Everything between the load and that rounding is fp32.  Bound by HBM: every value is read and written once.
 #include <cuda_bf16.h>
+#include <type_traits>
 #include "front.h"
 #include "ptx.cuh"
 
@@ -89,33 +90,237 @@ struct RotateParams {
     RotateSide side[2];
     const float* cos_sin;
     const int32_t* positions;
-    int64_t rows;          // tokens x (heads of queries + of keys)
+    int64_t units;         // tokens x chunks of heads
+    int q_chunks, chunks;  // of a token: those of queries, all
     int q_heads, heads, head_dim, rope_begin, rope_dim, max_positions, interleaved, center;
-    float eps;
+    float eps, inv_dim;
 };
 
-// kLanes lanes take a row; a lane holds kVecs times eight consecutive values.
-template <typename In, bool kE4m3, int kLanes, int kVecs>
-__global__ void __launch_bounds__(256) norm_rotate_kernel(const __grid_constant__ RotateParams p) {
-    const int lane = threadIdx.x % kLanes;
-    const int64_t row = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-    bool live = row < p.rows;
-    const int64_t token = live ? row / p.heads : 0;
-    int head = live ? (int)(row - token * p.heads) : 0;
-    const RotateSide& s = p.side[head >= p.q_heads ? 1 : 0];
-    const bool is_q = head < p.q_heads;
-    if (!is_q) head -= p.q_heads;
-    int pos = 0;
-    if (live && p.positions != nullptr) {
-        pos = __ldg(p.positions + token);
-        live = pos >= 0 && pos < p.max_positions;
+// What a group of lanes works on: kHeads heads of one token's queries or keys.
+struct RotateUnit {
+    int64_t token;
+    int head, count, pos;
+    bool is_q, live;
+};
+template <int kHeads> __device__ __forceinline__ RotateUnit unit_of(const RotateParams& p, int64_t unit) {
+    RotateUnit u;
+    u.live = unit < p.units;
+    if (!u.live) unit = 0;
+    if (p.units <= 0x7FFFFFFF) u.token = (uint32_t)unit / (uint32_t)p.chunks;   // (a 64-bit division is a hundred instructions)
+    else u.token = unit / p.chunks;
+    int chunk = (int)(unit - u.token * p.chunks);
+    u.is_q = chunk < p.q_chunks;
+    if (!u.is_q) chunk -= p.q_chunks;
+    u.head = chunk * kHeads;
+    u.count = min(kHeads, (u.is_q ? p.q_heads : p.heads - p.q_heads) - u.head);
+    u.pos = 0;
+    if (u.live && p.positions != nullptr) {
+        u.pos = __ldg(p.positions + u.token);
+        u.live = u.pos >= 0 && u.pos < p.max_positions;
     }
-    const In* x = reinterpret_cast<const In*>(s.x) + token * s.x_row + head * s.x_head;
+    if (!u.live) u.count = 0;
+    return u;
+}
+// Subtracts the mean (center) and returns 1 / sqrt(mean of the squares + eps) (rsqrtf: two units in the last place).  Values behind the vector
+// stay zeros.
+template <int kLanes> __device__ __forceinline__ float centred_rstd(float (&v)[8], bool inside, float inv_dim, bool center, float eps) {
+    if (center) {
+        const float mean = sum_over<kLanes>(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]))) * inv_dim;
+        if (inside)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] -= mean;
+    }
+    float t = 0.0f, u = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        t = fmaf(v[i], v[i], t);
+        u = fmaf(v[i + 1], v[i + 1], u);
+    }
+    return rsqrtf(fmaf(sum_over<kLanes>(t + u), inv_dim, eps));
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* out, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(out) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+// The scale of a vector, and its values over it: eight products with a reciprocal (within a unit in the last place of 1 / scale) where the scale
+// is an ordinary number, else quotients.
+__device__ __forceinline__ float scale_of(float amax) {
+    if (!(amax >= 0x1p-90f && amax <= 0x1p90f)) return amax > 0.0f ? __fdiv_rn(amax, 448.0f) : 1.0f;
+    constexpr float r = 1.0f / 448.0f;
+    const float q = amax * r;
+    return __fmaf_rn(__fmaf_rn(-q, 448.0f, amax), r, q);   // the rounded quotient (Markstein, as in merge_pack.cu)
+}
+__device__ __noinline__ uint2 divide8(float a, float b, float c, float d, float e, float f, float g, float h, float scale) {
+    return make_uint2(e4m3x4(__fdiv_rn(a, scale), __fdiv_rn(b, scale), __fdiv_rn(c, scale), __fdiv_rn(d, scale)),
+                      e4m3x4(__fdiv_rn(e, scale), __fdiv_rn(f, scale), __fdiv_rn(g, scale), __fdiv_rn(h, scale)));
+}
+__device__ __forceinline__ uint2 pack8(const float (&v)[8], float scale) {
+    if (!(scale >= 0x1p-100f && scale <= 0x1p100f)) return divide8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], scale);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));
+    r = fmaf(fmaf(-scale, r, 1.0f), r, r);
+    return make_uint2(e4m3x4(v[0] * r, v[1] * r, v[2] * r, v[3] * r), e4m3x4(v[4] * r, v[5] * r, v[6] * r, v[7] * r));
+}
+__device__ __forceinline__ void put_scale(const RotateSide& s, int64_t at, float scale) { s.scale[at] = s.gate != nullptr ? scale * __ldg(s.gate + at) : scale; }
+
+// Eight values as they come: one 16-byte load of bf16, or two loads, the second `apart` values further on.
+template <typename In, bool kPairs> struct Raw;
+template <> struct Raw<__nv_bfloat16, true> {
+    uint4 u;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p, int64_t, bool there) {
+        u = make_uint4(0u, 0u, 0u, 0u);
+        if (there) u = __ldg(reinterpret_cast<const uint4*>(p));
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+};
+template <> struct Raw<__nv_bfloat16, false> {
+    uint2 a, b;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p, int64_t apart, bool there) {
+        a = b = make_uint2(0u, 0u);
+        if (there) {
+            a = __ldg(reinterpret_cast<const uint2*>(p));
+            b = __ldg(reinterpret_cast<const uint2*>(p + apart));
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const uint32_t w[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+};
+template <bool kPairs> struct Raw<float, kPairs> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p, int64_t apart, bool there) {
+        a = b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (there) {
+            a = __ldg(reinterpret_cast<const float4*>(p));
+            b = __ldg(reinterpret_cast<const float4*>(p + apart));
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const { v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w; }
+};
+
+// Vectors of up to 256 values: kLanes lanes a head, eight values a lane, kHeads heads of a token one after the other, all loaded first.  A lane's
+// values are consecutive ones where pairs of neighbours are turned (kPairs), else a lane of the rotated part has four of one half and the four
+// that they are turned against, so no value is exchanged.  Weights and angles of a lane's values stay in registers over the heads.
+template <typename In, bool kE4m3, int kLanes, int kHeads, bool kPairs, bool kNorm>
+__global__ void __launch_bounds__(256, kHeads == 1 ? 4 : 3) norm_rotate_kernel(const __grid_constant__ RotateParams p) {
+    grid_dependency_wait();
+    const int lane = threadIdx.x % kLanes;
+    const RotateUnit u = unit_of<kHeads>(p, (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes);
+    const RotateSide& s = p.side[u.is_q ? 0 : 1];
+    const bool inside = 8 * lane < p.head_dim;
+    const int count = inside ? u.count : 0;       // heads that this lane has values of
+    // the lane's values: four from c0 on, four from c1 on
+    const int half = p.rope_dim / 2;
+    int c0 = 8 * lane, c1 = c0 + 4, angle = -1;   // angle: its first pair of the table, -1: not turned
+    if (kPairs) {
+        if (c0 >= p.rope_begin && c0 < p.rope_begin + p.rope_dim) angle = (c0 - p.rope_begin) / 2;
+    } else if (c0 < p.rope_dim) {                 // the first lanes take the rotated part
+        angle = 4 * lane;
+        c0 = p.rope_begin + angle;
+        c1 = c0 + half;
+    } else if (c0 - p.rope_dim < p.rope_begin) {  // then what lies before it
+        c0 -= p.rope_dim;
+        c1 = c0 + 4;
+    }
+    const bool turns = angle >= 0 && count > 0;
+    const int64_t x_head = s.x_head, o_head = s.o_head;
+    const int64_t apart = kPairs ? 4 : c1 - c0;
+    const In* x = reinterpret_cast<const In*>(s.x) + u.token * s.x_row + u.head * x_head + c0;
+    Raw<In, kPairs> raw[kHeads];
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k, x += x_head) raw[k].load(x, apart, k < count);
+    const bool norm = kNorm && s.weight != nullptr, center = kNorm && norm && p.center, shifted = norm && s.bias != nullptr;
+    float w[8], co[4], si[4];
+    if (norm) {
+        Raw<float, kPairs> t;
+        t.load(s.weight + c0, apart, inside);         // (lanes behind the vector stay zero)
+        t.get(w);
+    }
+    if (turns) {
+        const float* table = p.cos_sin + (int64_t)u.pos * p.rope_dim + angle;
+        load4(table, co);
+        load4(table + half, si);
+    }
+    using Out = typename std::conditional<kE4m3, uint8_t, __nv_bfloat16>::type;
+    Out* out = reinterpret_cast<Out*>(s.out) + u.token * s.o_row + u.head * o_head + c0;
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k, out += o_head) {
+        float y[8];
+        raw[k].get(y);
+        if (kNorm) {
+            const float rstd = centred_rstd<kLanes>(y, inside, p.inv_dim, center, p.eps);   // (the whole warp, whichever side its heads are of)
+            if (norm) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = y[i] * rstd * w[i];
+                if (shifted) {
+                    float b[8];
+                    Raw<float, kPairs> t;
+                    t.load(s.bias + c0, apart, inside);
+                    t.get(b);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] += b[i];
+                }
+            }
+        }
+        if (turns)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int i0 = kPairs ? 2 * i : i, i1 = kPairs ? 2 * i + 1 : i + 4;
+                const float a = y[i0], e = y[i1];
+                y[i0] = a * co[i] - e * si[i];
+                y[i1] = a * si[i] + e * co[i];
+            }
+        if constexpr (kE4m3) {
+            float amax = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(y[i]));
+            const float scale = scale_of(max_over<kLanes>(amax));
+            const uint2 codes = pack8(y, scale);
+            if (k < count) {
+                if constexpr (kPairs) {
+                    *reinterpret_cast<uint2*>(out) = codes;
+                } else {
+                    *reinterpret_cast<uint32_t*>(out) = codes.x;
+                    *reinterpret_cast<uint32_t*>(out + apart) = codes.y;
+                }
+                if (lane == 0) put_scale(s, u.token * (u.is_q ? p.q_heads : p.heads - p.q_heads) + u.head + k, scale);
+            }
+        } else if (k < count) {
+            if constexpr (kPairs) {
+                store8(out, y);
+            } else {
+                *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+                *reinterpret_cast<uint2*>(out + apart) = make_uint2(pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+            }
+        }
+    }
+}
+
+// Longer vectors: a warp a head, kVecs times eight values a lane.
+template <typename In, bool kE4m3, int kVecs>
+__global__ void __launch_bounds__(256) norm_rotate_long_kernel(const __grid_constant__ RotateParams p) {
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31;
+    const RotateUnit u = unit_of<1>(p, (int64_t)blockIdx.x * 8 + threadIdx.x / 32);
+    const RotateSide& s = p.side[u.is_q ? 0 : 1];
+    const In* x = reinterpret_cast<const In*>(s.x) + u.token * s.x_row + u.head * s.x_head;
+    if (!u.live) return;   // (a whole warp)
     float v[kVecs][8];
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
-        const int c = 8 * (lane + k * kLanes);
-        if (live && c < p.head_dim) {
+        const int c = 8 * (lane + k * 32);
+        if (c < p.head_dim) {
             load8(x + c, v[k]);
         } else {
 #pragma unroll
@@ -124,37 +329,37 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(const __grid_constant_
     }
     float mean = 0.0f, rstd = 1.0f;
     const bool norm = s.weight != nullptr;
-    if (p.side[0].weight != nullptr || p.side[1].weight != nullptr) {   // (the whole warp, whichever side its rows are of)
+    if (norm) {
         if (p.center) {
             float t = 0.0f;
 #pragma unroll
             for (int k = 0; k < kVecs; ++k)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) t += v[k][i];
-            mean = sum_over<kLanes>(t) / (float)p.head_dim;
+            mean = sum_over<32>(t) * p.inv_dim;
         }
         float t = 0.0f;
 #pragma unroll
         for (int k = 0; k < kVecs; ++k)
-            if (8 * (lane + k * kLanes) < p.head_dim)
+            if (8 * (lane + k * 32) < p.head_dim)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) t = fmaf(v[k][i] - mean, v[k][i] - mean, t);
-        rstd = 1.0f / sqrtf(sum_over<kLanes>(t) / (float)p.head_dim + p.eps);
+        rstd = rsqrtf(fmaf(sum_over<32>(t), p.inv_dim, p.eps));
     }
-    auto normed = [&](float (&u)[8], int c) {
+    auto normed = [&](float (&y)[8], int c) {
         if (!norm) return;
         float w[8], b[8];
         load8(s.weight + c, w);
         if (s.bias != nullptr) load8(s.bias + c, b);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = (u[i] - mean) * rstd * w[i] + (s.bias != nullptr ? b[i] : 0.0f);
+        for (int i = 0; i < 8; ++i) y[i] = (y[i] - mean) * rstd * w[i] + (s.bias != nullptr ? b[i] : 0.0f);
     };
-    const float* table = p.cos_sin + (int64_t)pos * p.rope_dim;
+    const float* table = p.cos_sin + (int64_t)u.pos * p.rope_dim;
     const int half = p.rope_dim / 2;
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
-        const int c = 8 * (lane + k * kLanes);
-        if (!live || c >= p.head_dim) continue;
+        const int c = 8 * (lane + k * 32);
+        if (c >= p.head_dim) continue;
         normed(v[k], c);
         const int r = c - p.rope_begin;
         if (r < 0 || r >= p.rope_dim) continue;
@@ -185,45 +390,68 @@ __global__ void __launch_bounds__(256) norm_rotate_kernel(const __grid_constant_
         for (int k = 0; k < kVecs; ++k)
 #pragma unroll
             for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[k][i]));
-        const Divider d(max_over<kLanes>(amax));
-        if (!live) return;
-        uint8_t* out = reinterpret_cast<uint8_t*>(s.out) + token * s.o_row + head * s.o_head;
+        const float scale = scale_of(max_over<32>(amax));
+        uint8_t* out = reinterpret_cast<uint8_t*>(s.out) + u.token * s.o_row + u.head * s.o_head;
 #pragma unroll
         for (int k = 0; k < kVecs; ++k) {
-            const int c = 8 * (lane + k * kLanes);
-            if (c < p.head_dim)
-                *reinterpret_cast<uint2*>(out + c) = make_uint2(e4m3x4(d(v[k][0]), d(v[k][1]), d(v[k][2]), d(v[k][3])), e4m3x4(d(v[k][4]), d(v[k][5]), d(v[k][6]), d(v[k][7])));
+            const int c = 8 * (lane + k * 32);
+            if (c < p.head_dim) *reinterpret_cast<uint2*>(out + c) = pack8(v[k], scale);
         }
-        if (lane == 0) {
-            const int64_t at = token * (is_q ? p.q_heads : p.heads - p.q_heads) + head;
-            s.scale[at] = s.gate != nullptr ? d.scale * __ldg(s.gate + at) : d.scale;
-        }
+        if (lane == 0) put_scale(s, u.token * (u.is_q ? p.q_heads : p.heads - p.q_heads) + u.head, scale);
     } else {
         __syncwarp();   // in place: a lane's values may still be another's partners
-        if (!live) return;
-        __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(s.out) + token * s.o_row + head * s.o_head;
+        __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(s.out) + u.token * s.o_row + u.head * s.o_head;
 #pragma unroll
         for (int k = 0; k < kVecs; ++k) {
-            const int c = 8 * (lane + k * kLanes);
-            if (c < p.head_dim)
-                *reinterpret_cast<uint4*>(out + c) = make_uint4(pack_bf16x2(v[k][0], v[k][1]), pack_bf16x2(v[k][2], v[k][3]), pack_bf16x2(v[k][4], v[k][5]), pack_bf16x2(v[k][6], v[k][7]));
+            const int c = 8 * (lane + k * 32);
+            if (c < p.head_dim) store8(out + c, v[k]);
         }
     }
 }
 
-template <typename In, bool kE4m3> cudaError_t launch_rotate(const RotateParams& p, cudaStream_t stream) {
-    auto go = [&](auto kernel, int lanes) {
-        const int64_t blocks = (p.rows * lanes + 255) / 256;
-        if (blocks > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-        kernel<<<(unsigned)blocks, 256, 0, stream>>>(p);
-        return cudaGetLastError();
+// A launch that may begin while the one before it in the stream ends; the kernels wait for it before they read anything.
+template <typename P> cudaError_t launch_after(void (*kernel)(P), int64_t blocks, int threads, const P& p, cudaStream_t stream) {
+    if (blocks > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <typename In, bool kE4m3> cudaError_t launch_rotate(RotateParams& p, int64_t tokens, cudaStream_t stream) {
+    int sms = 0;
+    cudaError_t e = sm_count(&sms);
+    if (e != cudaSuccess) return e;
+    // Four heads a unit once there are threads enough for the device without (2048 an SM).
+    auto go = [&](auto one, auto four, int lanes) {
+        const bool many = four != nullptr && tokens * p.heads * lanes >= (int64_t)sms * 2048;
+        const int each = many ? 4 : 1;
+        p.q_chunks = (p.q_heads + each - 1) / each;
+        p.chunks = p.q_chunks + (p.heads - p.q_heads + each - 1) / each;
+        p.units = tokens * p.chunks;
+        return launch_after(many ? four : one, (p.units * lanes + 255) / 256, 256, p, stream);
     };
-    if (p.head_dim <= 64) return go(norm_rotate_kernel<In, kE4m3, 8, 1>, 8);
-    if (p.head_dim <= 128) return go(norm_rotate_kernel<In, kE4m3, 16, 1>, 16);
-    if (p.head_dim <= 256) return go(norm_rotate_kernel<In, kE4m3, 32, 1>, 32);
-    if (p.head_dim <= 512) return go(norm_rotate_kernel<In, kE4m3, 32, 2>, 32);
-    if (p.head_dim <= 768) return go(norm_rotate_kernel<In, kE4m3, 32, 3>, 32);
-    return go(norm_rotate_kernel<In, kE4m3, 32, 4>, 32);
+    using Kernel = void (*)(RotateParams);
+    if (p.head_dim <= 256) {
+        auto of = [&](auto pairs, auto normed) {
+            constexpr bool kPairs = decltype(pairs)::value, kNorm = decltype(normed)::value;
+            if (p.head_dim <= 64) return go(Kernel(norm_rotate_kernel<In, kE4m3, 8, 1, kPairs, kNorm>), Kernel(norm_rotate_kernel<In, kE4m3, 8, 4, kPairs, kNorm>), 8);
+            if (p.head_dim <= 128) return go(Kernel(norm_rotate_kernel<In, kE4m3, 16, 1, kPairs, kNorm>), Kernel(norm_rotate_kernel<In, kE4m3, 16, 4, kPairs, kNorm>), 16);
+            return go(Kernel(norm_rotate_kernel<In, kE4m3, 32, 1, kPairs, kNorm>), Kernel(norm_rotate_kernel<In, kE4m3, 32, 4, kPairs, kNorm>), 32);
+        };
+        const bool pairs = p.interleaved || p.rope_dim == 0;
+        if (p.side[0].weight != nullptr || p.side[1].weight != nullptr) return pairs ? of(std::true_type(), std::true_type()) : of(std::false_type(), std::true_type());
+        return pairs ? of(std::true_type(), std::false_type()) : of(std::false_type(), std::false_type());
+    }
+    if (p.head_dim <= 512) return go(Kernel(norm_rotate_long_kernel<In, kE4m3, 2>), Kernel(nullptr), 32);
+    if (p.head_dim <= 768) return go(Kernel(norm_rotate_long_kernel<In, kE4m3, 3>), Kernel(nullptr), 32);
+    return go(Kernel(norm_rotate_long_kernel<In, kE4m3, 4>), Kernel(nullptr), 32);
 }
 
 // ------------------------------------------------------------------ append to the paged caches
@@ -255,6 +483,7 @@ __device__ __forceinline__ int64_t append_row(const AppendParams& p, int t, int 
 // One warp a row.  Units 0 .. tokens - 1 are rows of the attention's cache (when it is given), then those of the index cache.
 template <typename In, bool kFp8>
 __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
+    grid_dependency_wait();
     const int lane = threadIdx.x & 31;
     const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int n = p.a.num_tokens, n_kv = p.a.kv != nullptr ? n : 0;
@@ -294,7 +523,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
             for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) t2 = fmaf(v[k][i], v[k][i], t2);
-            const float rstd = 1.0f / sqrtf(sum_over<32>(t2) / (float)kDV + p.a.eps);
+            const float rstd = rsqrtf(fmaf(sum_over<32>(t2), 1.0f / kDV, p.a.eps));
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 float w[8];
@@ -330,11 +559,11 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
         load4(reinterpret_cast<const In*>(p.a.index_key) + t * p.a.stride_index_key + 4 * lane, v);
         if (p.a.index_weight != nullptr) {
             float mean = 0.0f;
-            if (p.a.index_center) mean = sum_over<32>((v[0] + v[1]) + (v[2] + v[3])) / (float)kDIndex;
+            if (p.a.index_center) mean = sum_over<32>((v[0] + v[1]) + (v[2] + v[3])) * (1.0f / kDIndex);
             float t2 = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) t2 = fmaf(v[i] - mean, v[i] - mean, t2);
-            const float rstd = 1.0f / sqrtf(sum_over<32>(t2) / (float)kDIndex + p.a.eps);
+            const float rstd = rsqrtf(fmaf(sum_over<32>(t2), 1.0f / kDIndex, p.a.eps));
             float w[4], b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             load4(p.a.index_weight + 4 * lane, w);
             if (p.a.index_bias != nullptr) load4(p.a.index_bias + 4 * lane, b);
@@ -385,7 +614,6 @@ cudaError_t launch_norm_rotate(const dsa_v32_norm_rotate_args& a, cudaStream_t s
     p.positions = a.positions;
     p.q_heads = a.q_heads;
     p.heads = a.q_heads + a.k_heads;
-    p.rows = (int64_t)a.num_tokens * p.heads;
     p.head_dim = a.head_dim;
     p.rope_begin = a.rope_begin;
     p.rope_dim = a.rope_dim;
@@ -393,7 +621,8 @@ cudaError_t launch_norm_rotate(const dsa_v32_norm_rotate_args& a, cudaStream_t s
     p.interleaved = a.interleaved;
     p.center = a.center;
     p.eps = a.eps;
-    if (p.rows == 0) return cudaSuccess;
+    p.inv_dim = 1.0f / (float)a.head_dim;
+    if (a.num_tokens == 0) return cudaSuccess;
     // In place and without a norm only the rotated values change: they are taken as the whole vectors.
     bool same = a.in_dtype == DSA_V32_DTYPE_BF16 && a.out_dtype == DSA_V32_DTYPE_BF16;
     for (int i = 0; i < 2; ++i) {
@@ -410,8 +639,8 @@ cudaError_t launch_norm_rotate(const dsa_v32_norm_rotate_args& a, cudaStream_t s
         p.rope_begin = 0;
     }
     const bool e4m3 = a.out_dtype == DSA_V32_DTYPE_E4M3;
-    if (a.in_dtype == DSA_V32_DTYPE_FP32) return e4m3 ? launch_rotate<float, true>(p, stream) : launch_rotate<float, false>(p, stream);
-    return e4m3 ? launch_rotate<__nv_bfloat16, true>(p, stream) : launch_rotate<__nv_bfloat16, false>(p, stream);
+    if (a.in_dtype == DSA_V32_DTYPE_FP32) return e4m3 ? launch_rotate<float, true>(p, a.num_tokens, stream) : launch_rotate<float, false>(p, a.num_tokens, stream);
+    return e4m3 ? launch_rotate<__nv_bfloat16, true>(p, a.num_tokens, stream) : launch_rotate<__nv_bfloat16, false>(p, a.num_tokens, stream);
 }
 
 cudaError_t launch_append(const dsa_v32_append_args& a, cudaStream_t stream) {
@@ -420,12 +649,10 @@ cudaError_t launch_append(const dsa_v32_append_args& a, cudaStream_t stream) {
         if (a.page_block_size == (1 << sh)) p.page_shift = sh;
     const int64_t units = (int64_t)a.num_tokens * ((a.kv != nullptr) + (a.index_cache != nullptr));
     if (units == 0) return cudaSuccess;
-    const unsigned blocks = (unsigned)((units + 7) / 8);
     const bool fp8 = a.kv_dtype == DSA_V32_KV_FP8;
-    auto kernel = a.in_dtype == DSA_V32_DTYPE_FP32 ? (fp8 ? append_kernel<float, true> : append_kernel<float, false>)
+    const auto kernel = a.in_dtype == DSA_V32_DTYPE_FP32 ? (fp8 ? append_kernel<float, true> : append_kernel<float, false>)
                                                    : (fp8 ? append_kernel<__nv_bfloat16, true> : append_kernel<__nv_bfloat16, false>);
-    kernel<<<blocks, 256, 0, stream>>>(p);
-    return cudaGetLastError();
+    return launch_after(kernel, (units + 7) / 8, 256, p, stream);
 }
 
 }  // namespace dsa
