@@ -28,6 +28,7 @@ constexpr int kMaxStages = 12;
 constexpr int kMaxSlots = 8;
 constexpr int kSmemBytes = 227 * 1024;
 constexpr int kScaleBytes = kTile * 4;
+constexpr int kDealt = 1024;          // most groups whose tiles are dealt out evenly
 
 struct Control {
     uint64_t k_full[kMaxStages], k_empty[kMaxStages];
@@ -38,6 +39,9 @@ struct Control {
     int abort_flag;
     uint32_t page_ok[kMaxStages];     // per stage, a bit per page of the tile
     int valid[2][kMaxRows];
+    int sums[kWarps];                 // dealing the tiles out
+    int share, first_group, first_tile;   // this CTA's tiles, and where they begin
+    int filled;                       // items whose unseen columns some warp has taken
     float best[4][2][4];              // what is exchanged: per warpgroup, twice, the warps' own largest
 };
 constexpr int kControlBytes = 1024;
@@ -53,7 +57,8 @@ struct Params {
     int64_t stride_w_row, stride_o_row, num_pages, seq_stride_pages;
     int H, s_q, kv_len, limit, block, block_shift, cols, block_table_stride, page_shift;
     int per, groups_per_seq, groups;      // query rows of a group, groups of a sequence and of all
-    int tiles, chunk, items;
+    int tiles, chunk, items;              // items: groups x chunks of tiles
+    int even;                             // the tiles of all groups are dealt out evenly
     int acc_cols, slots;                  // narrow: TMEM columns of an accumulator, accumulators in TMEM
     int stages, q_bufs;
     uint32_t off_k, off_s, off_w, q_bytes;   // shared memory: Q buffers | keys | their scales | weights | control
@@ -107,22 +112,111 @@ __device__ __forceinline__ void umma_f8_ss_x4_el(uint32_t d_tmem, uint32_t a_lo,
         : "memory");
 }
 
-// A work item.  Every role derives it by itself.
+// A work item: tiles of one group.
 struct Item {
     int seq, q0, rows, tile0, tiles;   // tiles: those that hold a position of some row
 };
 __device__ __forceinline__ int row_limit(const Params& p, int q) { return p.valid_len != nullptr ? max(0, min(p.limit, __ldg(p.valid_len + q))) : p.limit; }
-__device__ __forceinline__ Item item_of(const Params& p, int u, int lane) {
-    Item it;
-    const int c = u / p.groups, g = u - c * p.groups;
+__device__ __forceinline__ void group_of(const Params& p, int g, Item& it) {
     it.seq = g / p.groups_per_seq;
     const int r0 = (g - it.seq * p.groups_per_seq) * p.per;
     it.q0 = it.seq * p.s_q + r0;
     it.rows = min(p.per, p.s_q - r0);
+}
+// tiles of the group that hold a position of some row: one warp
+__device__ __forceinline__ int live_tiles(const Params& p, const Item& it, int lane) {
+    return (__reduce_max_sync(0xffffffffu, lane < it.rows ? row_limit(p, it.q0 + lane) : 0) + kTile - 1) / kTile;
+}
+// item u of the groups x chunks
+__device__ __forceinline__ Item item_of(const Params& p, int u, int lane) {
+    Item it;
+    const int c = u / p.groups;
+    group_of(p, u - c * p.groups, it);
     it.tile0 = c * p.chunk;
-    const int n = __reduce_max_sync(0xffffffffu, lane < it.rows ? row_limit(p, it.q0 + lane) : 0);
-    it.tiles = max(0, min((n + kTile - 1) / kTile - it.tile0, min(p.chunk, p.tiles - it.tile0)));
+    it.tiles = max(0, min(live_tiles(p, it, lane) - it.tile0, min(p.chunk, p.tiles - it.tile0)));
     return it;
+}
+// The items of a CTA, walked by every role for itself.  Few groups (a decode batch of ragged lengths): the CTA's share of all tiles, counted
+// through the groups.  Many: every gridDim-th of groups x chunks.
+struct Walk {
+    const Params& p;
+    int left, g, t, u, lane;
+    __device__ __forceinline__ Walk(const Params& p_, const Control* ctl, int lane_)
+        : p(p_), left(ctl->share), g(ctl->first_group), t(ctl->first_tile), u(blockIdx.x), lane(lane_) {}
+    __device__ __forceinline__ bool next(Item& it) {   // false: no more
+        if (p.even) {
+            while (left > 0) {
+                group_of(p, g++, it);
+                it.tile0 = t;
+                it.tiles = min(live_tiles(p, it, lane) - t, left);
+                t = 0;
+                if (it.tiles <= 0) continue;
+                left -= it.tiles;
+                return true;
+            }
+            return false;
+        }
+        while (u < p.items) {
+            it = item_of(p, u, lane);
+            u += gridDim.x;
+            if (it.tiles > 0) return true;
+        }
+        return false;
+    }
+};
+// All threads of the CTA: its share.
+__device__ void deal_out(const Params& p, Control* ctl) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, each = (p.groups + 32 * kWarps - 1) / (32 * kWarps);
+    const int g0 = min(tid * each, p.groups), g1 = min(g0 + each, p.groups);
+    auto tiles_of = [&](int g) {
+        Item it;
+        group_of(p, g, it);
+        int n = 0;
+        for (int r = 0; r < it.rows; ++r) n = max(n, row_limit(p, it.q0 + r));
+        return (n + kTile - 1) / kTile;
+    };
+    int sum = 0;
+    for (int g = g0; g < g1; ++g) sum += tiles_of(g);
+    int incl = sum;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += o;
+    }
+    if (lane == 31) ctl->sums[warp] = incl;
+    __syncthreads();
+    int before = incl - sum, all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += ctl->sums[w];
+        all += ctl->sums[w];
+    }
+    const int lo = (int)((int64_t)all * blockIdx.x / gridDim.x), hi = (int)((int64_t)all * (blockIdx.x + 1) / gridDim.x);
+    if (tid == 0) ctl->share = hi - lo;
+    if (lo >= before && lo < before + sum) {   // one thread, when there is a tile at all
+        int g = g0, n = 0;
+        for (; before + (n = tiles_of(g)) <= lo; ++g) before += n;
+        ctl->first_group = g;
+        ctl->first_tile = lo - before;
+    }
+    __syncthreads();
+}
+// One warp: value into columns of tiles [tile0, tile1) of the item's rows.
+__device__ __forceinline__ void fill(const Params& p, const Item& it, int tile0, int tile1, float value, int lane) {
+    const int c0 = (int)((int64_t)tile0 * kTile / p.block), c1 = (int)min((int64_t)p.cols, (int64_t)tile1 * kTile / p.block);
+    for (int r = 0; r < it.rows; ++r)
+        for (int c = c0 + lane; c < c1; c += 32) p.out[(int64_t)(it.q0 + r) * p.stride_o_row + c] = value;
+}
+// The columns behind the last position that a row of an item sees; whichever warp has nothing else to do takes the next item of the CTA's.
+__device__ __forceinline__ void fill_unseen(const Params& p, Control* ctl, int lane) {
+    while (true) {
+        int n = 0;
+        if (lane == 0) n = atomicAdd(&ctl->filled, 1);
+        n = __shfl_sync(0xffffffffu, n, 0);
+        const int64_t u = blockIdx.x + (int64_t)n * gridDim.x;
+        if (u >= p.items) return;
+        const Item it = item_of(p, (int)u, lane);
+        fill(p, it, it.tile0 + it.tiles, min(it.tile0 + p.chunk, p.tiles), -INFINITY, lane);
+    }
 }
 
 // ------------------------------------------------ sums over heads
@@ -246,6 +340,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
         }
         for (int i = 0; i < 4; ++i) mbar_init(bar_at(offsetof(Control, exchange), i), 4);
         ctl->abort_flag = 0;
+        ctl->share = ctl->first_group = ctl->first_tile = ctl->filled = 0;
         fence_mbar_init();
     }
     if (warp == kEpiWarps && lane == 0) {
@@ -261,6 +356,9 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
     tc_fence_after();
     const uint32_t tmem = ctl->tmem_base;
     grid_dependency_wait();
+    if (p.even) deal_out(p, ctl);
+    Walk walk(p, ctl, lane);
+    Item it;
 
     if (warp < kEpiWarps) {
         // ------------------------------------------------ scores out
@@ -271,7 +369,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
         Ring k, acc, wb;
         uint32_t exchanges = 0;
         bool ok = true;
-        int u = blockIdx.x;
+        int done = 0;      // items
         // A score to its place: s of position pos, -inf unless it counts; `stored`: the row is one.
         auto put = [&](float s, bool counts, int pos, float* at, bool stored) {
             s = counts ? s : -INFINITY;
@@ -316,9 +414,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
             constexpr int kRows = 128 / kCols;                         // of a warpgroup: half of an accumulator
             const int half = wg >> 1, row0 = wg * kRows;
             const uint32_t at = lanes + row0 * kCols, full = bar_at(offsetof(Control, acc_full), half), empty = bar_at(offsetof(Control, acc_empty), half);
-            for (; u < p.items && ok; u += gridDim.x) {
-                const Item it = item_of(p, u, lane);
-                if (it.tiles == 0) continue;
+            for (; ok && walk.next(it); ++done) {
                 if (!(ok = wait(bar_at(offsetof(Control, w_full), wb.s), wb.ph, abort_flag))) break;
                 int pos = it.tile0 * kTile + mine, end[kRows];
                 const uint32_t w = base + p.off_w + wb.s * p.per * kCols * 4 + 16 * (lane & 3) + row0 * kCols * 4;
@@ -355,9 +451,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
             int turn = wg;                     // tiles until this warpgroup's next one
             k.skip(wg, p.stages);
             acc.skip(wg, p.slots);
-            for (; u < p.items && ok; u += gridDim.x) {
-                const Item it = item_of(p, u, lane);
-                if (it.tiles == 0) continue;
+            for (; ok && walk.next(it); ++done) {
                 if (!(ok = wait(bar_at(offsetof(Control, w_full), wb.s), wb.ph, abort_flag))) break;
                 int i = turn;
                 for (; i < it.tiles && ok; i += 4, k.skip(4, p.stages), acc.skip(4, p.slots)) {
@@ -385,24 +479,17 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
                 wb.next(p.q_bufs);
             }
         }
-        // The columns behind the last position that a row of an item sees, once nothing waits for this warp any more.  After a wait that
-        // gave up: all of the items that were not finished.
-        for (int v = blockIdx.x; v < p.items; v += gridDim.x) {
-            const Item it = item_of(p, v, lane);
-            const bool lost = !ok && v >= u;
-            const int from = it.tile0 + (lost ? 0 : it.tiles), to = min(it.tile0 + p.chunk, p.tiles);
-            const int c0 = (int)((int64_t)from * kTile / p.block), c1 = (int)min((int64_t)p.cols, (int64_t)to * kTile / p.block);
-            for (int r = 0; r < it.rows; ++r)
-                for (int c = c0 + (lost ? lane : tid); c < c1; c += lost ? 32 : 32 * kEpiWarps)
-                    p.out[(int64_t)(it.q0 + r) * p.stride_o_row + c] = lost ? __int_as_float(0x7FFFFFFF) : -INFINITY;
+        if (!ok) {   // a wait gave up: every warp that saw it marks all of the items that were not finished
+            Walk again(p, ctl, lane);
+            for (int n = 0; again.next(it); ++n)
+                if (n >= done) fill(p, it, it.tile0, it.tile0 + it.tiles, __int_as_float(0x7FFFFFFF), lane);
         }
     } else if (warp == kEpiWarps) {
         // ------------------------------------------------ keys in
         Ring k;
         const int page_rows = 1 << min(p.page_shift, 7), pages = kTile / page_rows;   // of a tile
         bool ok = true;
-        for (int u = blockIdx.x; u < p.items && ok; u += gridDim.x) {
-            const Item it = item_of(p, u, lane);
+        while (ok && walk.next(it)) {
             // Page numbers come 32 at a time, a batch ahead of their use (a load of them per tile was 700 clocks of every tile).
             const int per_batch = 32 / pages;   // tiles of a batch
             auto batch = [&](int first) {
@@ -447,9 +534,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
         // ------------------------------------------------ query rows, weights, lengths in
         Ring b;
         bool ok = true;
-        for (int u = blockIdx.x; u < p.items && ok; u += gridDim.x) {
-            const Item it = item_of(p, u, lane);
-            if (it.tiles == 0) continue;
+        while (ok && walk.next(it)) {
             if (!(ok = wait(bar_at(offsetof(Control, q_empty), b.s), b.ph ^ 1u, abort_flag))) break;
             const uint32_t bar = bar_at(offsetof(Control, q_full), b.s), dst = smem_u32(smem) + b.s * p.q_bytes;
             if (lane == 0) mbar_arrive_expect_tx(bar, it.rows * kCols * (kFp8 ? 128 : 256));
@@ -475,9 +560,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
         const uint32_t el = elect_one() ? 1u : 0u;
         const uint64_t k_desc = make_smem_desc_sw128(smem_u32(k_smem), 0, 1024), q_desc = make_smem_desc_sw128(smem_u32(smem), 0, 1024);
         const uint32_t k_lo = (uint32_t)k_desc, q_lo = (uint32_t)q_desc, hi = (uint32_t)(k_desc >> 32);
-        for (int u = blockIdx.x; u < p.items && ok; u += gridDim.x) {
-            const Item it = item_of(p, u, lane);
-            if (it.tiles == 0) continue;
+        while (ok && walk.next(it)) {
             if (!(ok = wait(bar_at(offsetof(Control, q_full), b.s), b.ph, abort_flag))) break;
             for (int i = 0; i < it.tiles && ok; ++i, k.next(p.stages)) {
                 if (!(ok = wait(bar_at(offsetof(Control, k_full), k.s), k.ph, abort_flag))) break;
@@ -507,6 +590,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
         }
     }
     __syncwarp();
+    if (warp != kWarps - 1) fill_unseen(p, ctl, lane);
     tc_fence_before();
     __syncthreads();
     if (ctl->abort_flag) {
@@ -603,7 +687,7 @@ cudaError_t launch_index_scores(const dsa_v32_index_scores_args& a, const CUtens
     p.off_k = p.q_bufs * p.q_bytes;
     p.off_s = p.off_k + p.stages * (fp8 ? kKeyBytes<true> : kKeyBytes<false>);
     p.off_w = p.off_k + p.stages * stage;
-    // tiles of an item: the least for the busiest CTA, an item counted as two tiles more
+    // tiles of an item: the least for the busiest CTA, an item counted as two tiles more (for few groups the items are only what is filled)
     p.tiles = (a.kv_len + kTile - 1) / kTile;
     int64_t best = 0, items = 0;
     for (int c = 1; c <= p.tiles; c = c < 8 ? c + 1 : c + c / 4) {
@@ -618,7 +702,9 @@ cudaError_t launch_index_scores(const dsa_v32_index_scores_args& a, const CUtens
     if (items == 0) return cudaErrorInvalidConfiguration;
     p.groups = (int)groups;
     p.items = (int)items;
-    const int grid = (int)(items < sms ? items : sms);
+    const int64_t most_tiles = groups * p.tiles;
+    p.even = groups <= kDealt && most_tiles <= 0x7FFFFFFF;
+    const int grid = (int)(p.even ? (most_tiles < sms ? most_tiles : sms) : (items < sms ? items : sms));
     const bool all = a.H == cols;
     auto go = [&](auto kernel) { return kernel(tk, tq, p, grid, stream); };
 #define DSA_SCORES_OF(fp8_, cols_)                                                                                       \
