@@ -54,21 +54,6 @@ template <int kLanes> __device__ __forceinline__ float max_over(float x) {
     return x;
 }
 
-// Quotients by one scale, each the rounded quotient (the steps of pack_fp8_rows_kernel in merge_pack.cu).
-struct Divider {
-    float scale, recip;
-    bool plain;
-    __device__ explicit Divider(float amax) {
-        scale = amax > 0.0f ? __fdiv_rn(amax, 448.0f) : 1.0f;
-        recip = __frcp_rn(scale);
-        plain = scale >= 0x1p-80f && scale <= 0x1p80f;
-    }
-    __device__ float operator()(float a) const {
-        if (!plain) return __fdiv_rn(a, scale);
-        const float q = __fmul_rn(a, recip);
-        return copysignf(__fmaf_rn(__fmaf_rn(-q, scale, a), recip, q), a);
-    }
-};
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     uint16_t lo, hi;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
@@ -458,6 +443,7 @@ template <typename In, bool kE4m3> cudaError_t launch_rotate(RotateParams& p, in
 struct AppendParams {
     dsa_v32_append_args a;
     int page_shift;      // log2(page_block_size), or -1
+    int latent_warps;
 };
 
 // The physical row of a token, or -1: padding, or outside the table or the cache.
@@ -480,127 +466,252 @@ __device__ __forceinline__ int64_t append_row(const AppendParams& p, int t, int 
     return row < p.a.num_kv_rows ? row : -1;
 }
 
-// One warp a row.  Units 0 .. tokens - 1 are rows of the attention's cache (when it is given), then those of the index cache.
-template <typename In, bool kFp8>
-__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
-    grid_dependency_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int n = p.a.num_tokens, n_kv = p.a.kv != nullptr ? n : 0;
-    if (unit >= (int64_t)n_kv + (p.a.index_cache != nullptr ? n : 0)) return;
-    const bool index = unit >= n_kv;
-    const int t = (int)(index ? unit - n_kv : unit);
-    const int pos = __ldg(p.a.positions + t);
-    const int64_t row = append_row(p, t, pos);
-    if (row < 0) return;
-    const float* table = p.a.cos_sin + (int64_t)pos * kDRope;
-
-    if (!index) {
-        // lane = eight of them a group of 128 values: 16 values each, and two of the rope key
-        const In* x = reinterpret_cast<const In*>(p.a.latent) + t * p.a.stride_latent + 16 * lane;
-        float v[2][8];
-        load8(x, v[0]);
-        load8(x + 8, v[1]);
-        const In* r = reinterpret_cast<const In*>(p.a.rope) + t * p.a.stride_rope;
-        uint32_t rope;
-        if (p.a.interleaved) {
-            float u[2];
-            load2(r + 2 * lane, u);
-            const float co = __ldg(table + lane), si = __ldg(table + 32 + lane);
-            rope = pack_bf16x2(u[0] * co - u[1] * si, u[0] * si + u[1] * co);
-        } else {
-            const bool upper = lane >= 16;
-            float u[2], o[2], co[2], si[2];
-            load2(r + 2 * lane, u);
-            load2(r + 2 * (lane ^ 16), o);
-            load2(table + 2 * (lane & 15), co);
-            load2(table + 32 + 2 * (lane & 15), si);
-            rope = upper ? pack_bf16x2(o[0] * si[0] + u[0] * co[0], o[1] * si[1] + u[1] * co[1]) : pack_bf16x2(u[0] * co[0] - o[0] * si[0], u[1] * co[1] - o[1] * si[1]);
+// Eight values over their scale as e4m3, each the rounded quotient (one step of Newton and one of Markstein, as in merge_pack.cu), two at a time.
+// n: the values negated, so that a zero keeps its sign: q = n (-1/s), then q - (q s + n) / s.
+__device__ __forceinline__ uint2 quotients8(const uint64_t (&n)[4], float scale) {
+    if (!(scale >= 0x1p-80f && scale <= 0x1p80f)) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) unpack2(n[i], v[2 * i], v[2 * i + 1]);
+        return divide8(-v[0], -v[1], -v[2], -v[3], -v[4], -v[5], -v[6], -v[7], scale);
+    }
+    const float r = -__frcp_rn(scale);
+    const uint64_t r2 = pack2(r, r), s2 = pack2(scale, scale);
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint64_t q = mul2(n[2 * i + j], r2);
+            unpack2(fma2(fma2(q, s2, n[2 * i + j]), r2, q), v[2 * j], v[2 * j + 1]);
         }
-        if (p.a.latent_weight != nullptr) {
-            float t2 = 0.0f;
+        w[i] = e4m3x4(v[0], v[1], v[2], v[3]);
+    }
+    return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ float amax2(uint64_t v, float m) {
+    float a, b;
+    unpack2(v, a, b);
+    return max3(m, fabsf(a), fabsf(b));
+}
+
+// The tokens of a warp: lane k resolves token first + k, and holds its position and row (-1: not written).
+struct Placed {
+    int pos, row;
+};
+template <int kTokens> __device__ __forceinline__ Placed place(const AppendParams& p, int first, int lane) {
+    Placed r{0, -1};
+    if (lane < kTokens && first + lane < p.a.num_tokens) {
+        r.pos = __ldg(p.a.positions + first + lane);
+        r.row = (int)append_row(p, first + lane, r.pos);
+    }
+    return r;
+}
+
+// Rows of the attention's cache: a warp a token, 16 values a lane (eight lanes a group of 128) and two of the rope key.  All inputs of the warp's
+// kTokens tokens are loaded before their places are known.
+template <typename In, bool kFp8, int kTokens> __device__ __forceinline__ void append_latents(const AppendParams& p, int first, int lane) {
+    const int n = p.a.num_tokens;
+    Raw<In, true> raw[kTokens][2];
+    float pe[kTokens][2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < kTokens; ++k) {
+        const int t = min(first + k, n - 1);
+        const In* x = reinterpret_cast<const In*>(p.a.latent) + t * p.a.stride_latent + 16 * lane;
+        raw[k][0].load(x, 4, true);
+        raw[k][1].load(x + 8, 4, true);
+        load2(reinterpret_cast<const In*>(p.a.rope) + t * p.a.stride_rope + 2 * lane, pe[k]);
+    }
+    const Placed at = place<kTokens>(p, first, lane);
+    const bool norm = p.a.latent_weight != nullptr;
+    uint64_t w[8];
+    if (norm) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t2 = fmaf(v[k][i], v[k][i], t2);
-            const float rstd = rsqrtf(fmaf(sum_over<32>(t2), 1.0f / kDV, p.a.eps));
+        for (int i = 0; i < 4; ++i) {
+            float f[4];
+            load4(p.a.latent_weight + 16 * lane + 4 * i, f);
+            w[2 * i] = pack2(f[0], f[1]);
+            w[2 * i + 1] = pack2(f[2], f[3]);
+        }
+    }
+    int row[kTokens];
+    float co[kTokens][2], si[kTokens][2];      // neighbours: one angle; halves: two
+    const bool pairs = p.a.interleaved;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                float w[8];
-                load8(p.a.latent_weight + 16 * lane + 8 * k, w);
+    for (int k = 0; k < kTokens; ++k) {
+        row[k] = __shfl_sync(0xffffffffu, at.row, k);
+        const int pos = __shfl_sync(0xffffffffu, at.pos, k);
+        if (row[k] < 0) continue;
+        const float* table = p.a.cos_sin + (int64_t)pos * kDRope;
+        if (pairs) {
+            co[k][0] = __ldg(table + lane), si[k][0] = __ldg(table + 32 + lane);
+        } else {
+            load2(table + 2 * (lane & 15), co[k]);
+            load2(table + 32 + 2 * (lane & 15), si[k]);
+        }
+    }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[k][i] = v[k][i] * rstd * w[i];
+    for (int k = 0; k < kTokens; ++k) {
+        if (row[k] < 0) continue;
+        uint32_t rope;
+        if (pairs) {
+            rope = pack_bf16x2(pe[k][0] * co[k][0] - pe[k][1] * si[k][0], pe[k][0] * si[k][0] + pe[k][1] * co[k][0]);
+        } else {
+            const float o0 = __shfl_xor_sync(0xffffffffu, pe[k][0], 16), o1 = __shfl_xor_sync(0xffffffffu, pe[k][1], 16);
+            rope = lane >= 16 ? pack_bf16x2(o0 * si[k][0] + pe[k][0] * co[k][0], o1 * si[k][1] + pe[k][1] * co[k][1])
+                              : pack_bf16x2(pe[k][0] * co[k][0] - o0 * si[k][0], pe[k][1] * co[k][1] - o1 * si[k][1]);
+        }
+        uint64_t v[8];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float f[8];
+            raw[k][j].get(f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * j + i] = pack2(f[2 * i], f[2 * i + 1]);
+        }
+        float factor = kFp8 ? -1.0f : 1.0f;        // (quotients8 takes them negated)
+        if (norm) {
+            uint64_t t0 = 0, t1 = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                t0 = fma2(v[i], v[i], t0);
+                t1 = fma2(v[i + 1], v[i + 1], t1);
             }
+            float a, b;
+            unpack2(add2(t0, t1), a, b);
+            factor *= rsqrtf(fmaf(sum_over<32>(a + b), 1.0f / kDV, p.a.eps));
+        }
+        if (kFp8 || norm) {
+            const uint64_t f2 = pack2(factor, factor);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = mul2(v[i], f2);
+        }
+        if (norm) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = mul2(v[i], w[i]);
         }
         if constexpr (kFp8) {
             float amax = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[k][i]));
-            const Divider d(max_over<8>(amax));
-            uint8_t* out = reinterpret_cast<uint8_t*>(p.a.kv) + row * kFp8RowBytes;
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = e4m3x4(d(v[k >> 1][4 * (k & 1)]), d(v[k >> 1][4 * (k & 1) + 1]), d(v[k >> 1][4 * (k & 1) + 2]), d(v[k >> 1][4 * (k & 1) + 3]));
-            reinterpret_cast<uint4*>(out)[lane] = make_uint4(w[0], w[1], w[2], w[3]);
-            if ((lane & 7) == 0) reinterpret_cast<float*>(out + kDV)[lane >> 3] = d.scale;
+            for (int i = 0; i < 8; ++i) amax = amax2(v[i], amax);
+            const float scale = scale_of(max_over<8>(amax));
+            const uint64_t lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
+            const uint2 a = quotients8(lo, scale), b = quotients8(hi, scale);
+            uint8_t* out = reinterpret_cast<uint8_t*>(p.a.kv) + (int64_t)row[k] * kFp8RowBytes;
+            reinterpret_cast<uint4*>(out)[lane] = make_uint4(a.x, a.y, b.x, b.y);
+            if ((lane & 7) == 0) reinterpret_cast<float*>(out + kDV)[lane >> 3] = scale;
             reinterpret_cast<uint32_t*>(out + kDV + 16)[lane] = rope;
         } else {
-            uint8_t* out = reinterpret_cast<uint8_t*>(p.a.kv) + row * (2 * kDQK);
+            uint8_t* out = reinterpret_cast<uint8_t*>(p.a.kv) + (int64_t)row[k] * (2 * kDQK);
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-                reinterpret_cast<uint4*>(out)[2 * lane + k] = make_uint4(pack_bf16x2(v[k][0], v[k][1]), pack_bf16x2(v[k][2], v[k][3]), pack_bf16x2(v[k][4], v[k][5]), pack_bf16x2(v[k][6], v[k][7]));
+            for (int j = 0; j < 2; ++j)
+                reinterpret_cast<uint4*>(out)[2 * lane + j] =
+                    make_uint4(pack_bf16x2_from2(v[4 * j]), pack_bf16x2_from2(v[4 * j + 1]), pack_bf16x2_from2(v[4 * j + 2]), pack_bf16x2_from2(v[4 * j + 3]));
             reinterpret_cast<uint32_t*>(out + 2 * kDV)[lane] = rope;
         }
-    } else {
-        // lane = values 4 lane .. 4 lane + 3; the first 16 lanes hold the rotated half
-        float v[4];
-        load4(reinterpret_cast<const In*>(p.a.index_key) + t * p.a.stride_index_key + 4 * lane, v);
-        if (p.a.index_weight != nullptr) {
-            float mean = 0.0f;
-            if (p.a.index_center) mean = sum_over<32>((v[0] + v[1]) + (v[2] + v[3])) * (1.0f / kDIndex);
-            float t2 = 0.0f;
+    }
+}
+
+// Rows of the index cache: sixteen lanes a token, four values from c0 and four from c1 a lane (as in norm_rotate_kernel), kTokens tokens a warp.
+template <typename In, bool kFp8, int kTokens> __device__ __forceinline__ void append_index_keys(const AppendParams& p, int first, int lane) {
+    constexpr int kEach = kTokens / 2;
+    const int n = p.a.num_tokens, l = lane & 15, mine = lane >> 4;
+    const bool pairs = p.a.index_interleaved, turns = l < 8;
+    const int c0 = pairs || !turns ? 8 * l : 4 * l, apart = pairs || !turns ? 4 : 32;
+    Raw<In, false> raw[kEach];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) t2 = fmaf(v[i] - mean, v[i] - mean, t2);
-            const float rstd = rsqrtf(fmaf(sum_over<32>(t2), 1.0f / kDIndex, p.a.eps));
-            float w[4], b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            load4(p.a.index_weight + 4 * lane, w);
-            if (p.a.index_bias != nullptr) load4(p.a.index_bias + 4 * lane, b);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = (v[i] - mean) * rstd * w[i] + b[i];
+    for (int k = 0; k < kEach; ++k)
+        raw[k].load(reinterpret_cast<const In*>(p.a.index_key) + min(first + 2 * k + mine, n - 1) * p.a.stride_index_key + c0, apart, true);
+    const Placed at = place<kTokens>(p, first, lane);
+    const bool norm = p.a.index_weight != nullptr, shifted = p.a.index_bias != nullptr;
+    float w[8], b[8];
+    if (norm) {
+        Raw<float, false> t;
+        t.load(p.a.index_weight + c0, apart, true);
+        t.get(w);
+        if (shifted) {
+            t.load(p.a.index_bias + c0, apart, true);
+            t.get(b);
         }
-        float o[4];
+    }
+    int row[kEach];
+    float co[kEach][4], si[kEach][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = __shfl_xor_sync(0xffffffffu, v[i], 8);   // 32 values on: the other half of the rotated ones
-        if (lane < 16) {
-            if (p.a.index_interleaved) {
-                float co[2], si[2];
-                load2(table + 2 * lane, co);
-                load2(table + 32 + 2 * lane, si);
+    for (int k = 0; k < kEach; ++k) {
+        row[k] = __shfl_sync(0xffffffffu, at.row, 2 * k + mine);
+        const int pos = __shfl_sync(0xffffffffu, at.pos, 2 * k + mine);
+        if (row[k] < 0 || !turns) continue;
+        const float* table = p.a.cos_sin + (int64_t)pos * kDRope + 4 * l;
+        load4(table, co[k]);
+        load4(table + 32, si[k]);
+    }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float a = v[2 * i], b = v[2 * i + 1];
-                    v[2 * i] = a * co[i] - b * si[i];
-                    v[2 * i + 1] = a * si[i] + b * co[i];
-                }
+    for (int k = 0; k < kEach; ++k) {
+        float y[8];
+        raw[k].get(y);
+        if (norm) {
+            const float rstd = centred_rstd<16>(y, true, 1.0f / kDIndex, p.a.index_center, p.a.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = y[i] * rstd * w[i];
+            if (shifted)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] += b[i];
+        }
+        if (turns && row[k] >= 0) {
+            auto turn = [&](float& a, float& e, int i) {
+                const float x = a;
+                a = x * co[k][i] - e * si[k][i];
+                e = x * si[k][i] + e * co[k][i];
+            };
+            if (pairs) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) turn(y[2 * i], y[2 * i + 1], i);
             } else {
-                float co[4], si[4];
-                load4(table + 4 * (lane & 7), co);
-                load4(table + 32 + 4 * (lane & 7), si);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = lane >= 8 ? o[i] * si[i] + v[i] * co[i] : v[i] * co[i] - o[i] * si[i];
+                for (int i = 0; i < 4; ++i) turn(y[i], y[4 + i], i);
             }
         }
         if constexpr (kFp8) {
-            const Divider d(max_over<32>(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])))));
-            const int64_t page = row / p.a.page_block_size, at = row - page * p.a.page_block_size;
-            uint8_t* base = reinterpret_cast<uint8_t*>(p.a.index_cache) + page * p.a.page_block_size * (kDIndex + 4);
-            reinterpret_cast<uint32_t*>(base + at * kDIndex)[lane] = e4m3x4(d(v[0]), d(v[1]), d(v[2]), d(v[3]));
-            if (lane == 0) reinterpret_cast<float*>(base + (int64_t)p.a.page_block_size * kDIndex)[at] = d.scale;
+            uint64_t v[4];
+            float amax = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = pack2(-y[2 * i], -y[2 * i + 1]);
+                amax = amax2(v[i], amax);
+            }
+            const float scale = scale_of(max_over<16>(amax));
+            const uint2 codes = quotients8(v, scale);
+            if (row[k] < 0) continue;
+            const int64_t page = row[k] >> p.page_shift;
+            const int in_page = row[k] & (p.a.page_block_size - 1);          // (a power of two: the index cache's pages are)
+            uint8_t* base = reinterpret_cast<uint8_t*>(p.a.index_cache) + ((page * (kDIndex + 4)) << p.page_shift);
+            uint8_t* out = base + in_page * kDIndex + c0;
+            *reinterpret_cast<uint32_t*>(out) = codes.x;
+            *reinterpret_cast<uint32_t*>(out + apart) = codes.y;
+            if (l == 0) reinterpret_cast<float*>(base + ((int64_t)kDIndex << p.page_shift))[in_page] = scale;
         } else {
-            reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(p.a.index_cache) + row * (2 * kDIndex))[lane] = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+            if (row[k] < 0) continue;
+            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.a.index_cache) + (int64_t)row[k] * kDIndex + c0;
+            *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+            *reinterpret_cast<uint2*>(out + apart) = make_uint2(pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
         }
+    }
+}
+
+// (Blocks of 256 threads: 14.8 instead of 12.5 us for 16384 tokens into the fp8 caches, the last ones leave SMs half empty.)
+constexpr int kAppendThreads = 128;
+// Warps 0 .. latent_warps - 1 take kTokens tokens' rows of the attention's cache each, the others twice as many (at least two) of the index cache.
+template <typename In, bool kFp8, int kTokens>
+__global__ void __launch_bounds__(kAppendThreads, 8) append_kernel(const __grid_constant__ AppendParams p) {
+    grid_dependency_wait();
+    constexpr int kKeys = 2 * kTokens;
+    const int lane = threadIdx.x & 31, n = p.a.num_tokens;
+    const int64_t warp = (int64_t)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
+    if (warp < p.latent_warps) {
+        append_latents<In, kFp8, kTokens>(p, (int)warp * kTokens, lane);
+    } else if (p.a.index_cache != nullptr && (warp - p.latent_warps) * kKeys < n) {
+        append_index_keys<In, kFp8, kKeys>(p, (int)(warp - p.latent_warps) * kKeys, lane);
     }
 }
 
@@ -644,15 +755,27 @@ cudaError_t launch_norm_rotate(const dsa_v32_norm_rotate_args& a, cudaStream_t s
 }
 
 cudaError_t launch_append(const dsa_v32_append_args& a, cudaStream_t stream) {
-    AppendParams p{a, -1};
+    AppendParams p{a, -1, 0};
     for (int sh = 0; sh < 31; ++sh)
         if (a.page_block_size == (1 << sh)) p.page_shift = sh;
-    const int64_t units = (int64_t)a.num_tokens * ((a.kv != nullptr) + (a.index_cache != nullptr));
-    if (units == 0) return cudaSuccess;
-    const bool fp8 = a.kv_dtype == DSA_V32_KV_FP8;
-    const auto kernel = a.in_dtype == DSA_V32_DTYPE_FP32 ? (fp8 ? append_kernel<float, true> : append_kernel<float, false>)
-                                                   : (fp8 ? append_kernel<__nv_bfloat16, true> : append_kernel<__nv_bfloat16, false>);
-    return launch_after(kernel, (units + 7) / 8, 256, p, stream);
+    if (a.num_tokens == 0) return cudaSuccess;
+    int sms = 0;
+    cudaError_t e = sm_count(&sms);
+    if (e != cudaSuccess) return e;
+    const bool fp8 = a.kv_dtype == DSA_V32_KV_FP8, wide = a.in_dtype == DSA_V32_DTYPE_FP32;
+    auto go = [&](auto kernel, int tokens) {
+        p.latent_warps = a.kv != nullptr ? (a.num_tokens + tokens - 1) / tokens : 0;
+        const int64_t warps = p.latent_warps + (a.index_cache != nullptr ? ((int64_t)a.num_tokens + 2 * tokens - 1) / (2 * tokens) : 0);
+        return launch_after(kernel, (warps + kAppendThreads / 32 - 1) / (kAppendThreads / 32), kAppendThreads, p, stream);
+    };
+    // Two tokens a warp (their loads in flight together, the weights read once) where warps of one token each are more than the device holds with
+    // their CTAs' ends: 4096 tokens 4.8 instead of 5.6 us, 1024 tokens 3.4 instead of 2.9.  (Four: 14.2 instead of 12.5 us for 16384 tokens.)
+    if (a.num_tokens < 16 * sms) {
+        if (wide) return fp8 ? go(append_kernel<float, true, 1>, 1) : go(append_kernel<float, false, 1>, 1);
+        return fp8 ? go(append_kernel<__nv_bfloat16, true, 1>, 1) : go(append_kernel<__nv_bfloat16, false, 1>, 1);
+    }
+    if (wide) return fp8 ? go(append_kernel<float, true, 2>, 2) : go(append_kernel<float, false, 2>, 2);
+    return fp8 ? go(append_kernel<__nv_bfloat16, true, 2>, 2) : go(append_kernel<__nv_bfloat16, false, 2>, 2);
 }
 
 }  // namespace dsa
