@@ -526,6 +526,7 @@ def append_cache(latent, rope, kv, cos_sin, positions, *, seq_ids=None, s_q=1, b
     latent_at = rope_at = kv_at = key_at = cache_at = latent_stride = rope_stride = key_stride = 0
     dtype = kind = None
     if kv is not None:
+        assert latent is not None and rope is not None
         dtype, width = latent.dtype, kv.shape[-1]
         (latent_stride, l1), (rope_stride, r1) = latent.stride(), rope.stride()
         assert latent.shape == (tokens, D_V) and rope.shape == (tokens, D_ROPE) and rope.dtype is dtype and l1 == 1 and r1 == 1 and kv.is_contiguous()
@@ -540,6 +541,7 @@ def append_cache(latent, rope, kv, cos_sin, positions, *, seq_ids=None, s_q=1, b
     else:
         assert latent is None and rope is None and latent_weight is None and index_cache is not None
     if index_cache is not None:
+        assert index_key is not None
         index_kind, index_rows = _index_rows(index_cache, page_block_size)
         key_stride, k1 = index_key.stride()
         assert index_key.shape == (tokens, D_INDEX) and k1 == 1

@@ -60,6 +60,7 @@ struct Params {
     int tiles, chunk, items;              // items: groups x chunks of tiles
     int even;                             // the tiles of all groups are dealt out evenly
     int acc_cols, slots;                  // narrow: TMEM columns of an accumulator, accumulators in TMEM
+    int fulls;                            // barriers that say an accumulator is full
     int stages, q_bufs;
     uint32_t off_k, off_s, off_w, q_bytes;   // shared memory: Q buffers | keys | their scales | weights | control
 };
@@ -328,8 +329,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
             mbar_init(bar_at(offsetof(Control, k_full), i), 1);
             mbar_init(bar_at(offsetof(Control, k_empty), i), 1 + (kWide ? kEpiWarps : 4));
         }
-        for (int i = 0; i < (kWide ? 2 : p.slots); ++i) {
-            mbar_init(bar_at(offsetof(Control, acc_full), i), 2);
+        for (int i = 0; i < p.fulls; ++i) mbar_init(bar_at(offsetof(Control, acc_full), i), 2);
+        for (int i = 0; i < p.slots; ++i) {
             mbar_init(bar_at(offsetof(Control, acc_empty), i), kWide ? kEpiWarps / 2 : 4);
         }
         for (int i = 0; i < 2; ++i) {
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * sub) << 16);
         const int mine = 32 * sub + lane_position(lane);   // of a tile's positions
         const int page_bit = mine >> min(p.page_shift, 7), block = p.block, kv_len = p.kv_len;
-        Ring k, acc, wb;
+        Ring k, acc, fl, wb;
         uint32_t exchanges = 0;
         bool ok = true;
         int done = 0;      // items
@@ -451,12 +452,13 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
             int turn = wg;                     // tiles until this warpgroup's next one
             k.skip(wg, p.stages);
             acc.skip(wg, p.slots);
+            fl.skip(wg, p.fulls);
             for (; ok && walk.next(it); ++done) {
                 if (!(ok = wait(bar_at(offsetof(Control, w_full), wb.s), wb.ph, abort_flag))) break;
                 int i = turn;
-                for (; i < it.tiles && ok; i += 4, k.skip(4, p.stages), acc.skip(4, p.slots)) {
+                for (; i < it.tiles && ok; i += 4, k.skip(4, p.stages), acc.skip(4, p.slots), fl.skip(4, p.fulls)) {
                     const int pos = (it.tile0 + i) * kTile + mine;
-                    if (!(ok = wait(bar_at(offsetof(Control, acc_full), acc.s), acc.ph, abort_flag))) break;
+                    if (!(ok = wait(bar_at(offsetof(Control, acc_full), fl.s), fl.ph, abort_flag))) break;
                     tc_fence_after();
                     uint32_t at = lanes + acc.s * p.acc_cols, w = base + p.off_w + wb.s * p.per * kCols * 4 + 16 * (lane & 3);
                     load_row(at);
@@ -555,7 +557,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
         }
     } else {
         // ------------------------------------------------ MMAs
-        Ring k, acc, b;
+        Ring k, acc, fl, b;
         bool ok = true;
         const uint32_t el = elect_one() ? 1u : 0u;
         const uint64_t k_desc = make_smem_desc_sw128(smem_u32(k_smem), 0, 1024), q_desc = make_smem_desc_sw128(smem_u32(smem), 0, 1024);
@@ -570,7 +572,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
                     tc_fence_after();
                     const int n = kWide ? kMmaCols : it.rows * kCols;   // (wide: rows that there are not are never read back)
                     const uint32_t a = k_lo + ((k.s * kKeyBytes<kFp8>) >> 4), q = q_lo + ((b.s * p.q_bytes + part * kMmaCols * 128) >> 4);
-                    const uint32_t d = tmem + acc.s * (kWide ? kMmaCols : p.acc_cols), full = bar_at(offsetof(Control, acc_full), acc.s);
+                    const uint32_t d = tmem + acc.s * (kWide ? kMmaCols : p.acc_cols), full = bar_at(offsetof(Control, acc_full), fl.s);
                     if constexpr (kFp8) {
                         umma_f8_ss_x4_el(d, a, hi, q, hi, make_idesc_e4m3(kTile, n), el);
                     } else {
@@ -580,7 +582,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
                     }
                     tc_commit_el(full, el);
                     if (el) mbar_arrive(full);
-                    acc.next(kWide ? 2 : p.slots);
+                    acc.next(p.slots);
+                    fl.next(p.fulls);
                 }
                 if (ok) tc_commit_el(bar_at(offsetof(Control, k_empty), k.s), el);
             }
@@ -678,6 +681,9 @@ cudaError_t launch_index_scores(const dsa_v32_index_scores_args& a, const CUtens
     p.acc_cols = 64;
     while (p.acc_cols < p.per * cols) p.acc_cols *= 2;
     p.slots = wide ? 2 : kTmemCols / p.acc_cols;
+    // Tiles go to four warpgroups in turn.  With two accumulators two of them share one, and a wait by parity must not be two phases ahead of its
+    // barrier, so every warpgroup has a full barrier of its own.
+    p.fulls = wide || p.slots > 4 ? p.slots : 4;
     // shared memory: two buffers of query rows where that leaves four stages of keys
     const int stage = fp8 ? kKeyBytes<true> + kScaleBytes : kKeyBytes<false>;
     p.q_bytes = p.per * cols * (fp8 ? 128 : 256);
