@@ -29,11 +29,6 @@ __device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
     const float4 a = __ldg(reinterpret_cast<const float4*>(p));
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
 }
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&v)[4]) {
-    const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-    v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xFFFF0000u);
-    v[2] = __uint_as_float(u.y << 16), v[3] = __uint_as_float(u.y & 0xFFFF0000u);
-}
 __device__ __forceinline__ void load2(const float* p, float (&v)[2]) {
     const float2 a = __ldg(reinterpret_cast<const float2*>(p));
     v[0] = a.x, v[1] = a.y;
