@@ -90,6 +90,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN where eith
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
+__device__ __forceinline__ float warp_max_nan(float a) {
+    float d;
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(a));
+    return d;
+}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
@@ -221,33 +226,50 @@ __device__ __forceinline__ void fill_unseen(const Params& p, Control* ctl, int l
 }
 
 // ------------------------------------------------ sums over heads
-// 16 lanes x kCols columns of an accumulator: thread t gets, for i < kCols / 8, columns 8 i + 2 (t % 4) and the next of lane t / 4 in
+// Twice 16 lanes x kCols columns of an accumulator: of either half thread t gets, for i < kCols / 8, columns 8 i + 2 (t % 4) and the next of lane t / 4 in
 // d[4 i], d[4 i + 1] and of lane t / 4 + 8 in d[4 i + 2], d[4 i + 3].  So a thread needs the weights of a quarter of the heads only (all of
 // them for every position, read from shared memory for every accumulator, were as many wavefronts as the MMAs' own operands and kept the
 // kernel at 1 800 cycles an accumulator), and the four threads of a quad add up their parts for four positions.
-template <int kCols> __device__ __forceinline__ void load_half(uint32_t taddr, uint32_t (&d)[kCols / 2]) {
+// The loads and their wait are one statement: with code between them (scores of the row before on their way out) an accumulator that was given back
+// behind the wait was overwritten before its upper half had been read.
+template <int kCols> __device__ __forceinline__ void load_row(uint32_t taddr, uint32_t (&lo)[kCols / 2], uint32_t (&hi)[kCols / 2]) {
     if constexpr (kCols == 64) {
         asm volatile(
-            "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
-            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-            "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7]), "=r"(d[8]), "=r"(d[9]), "=r"(d[10]), "=r"(d[11]),
-              "=r"(d[12]), "=r"(d[13]), "=r"(d[14]), "=r"(d[15]), "=r"(d[16]), "=r"(d[17]), "=r"(d[18]), "=r"(d[19]), "=r"(d[20]), "=r"(d[21]), "=r"(d[22]),
-              "=r"(d[23]), "=r"(d[24]), "=r"(d[25]), "=r"(d[26]), "=r"(d[27]), "=r"(d[28]), "=r"(d[29]), "=r"(d[30]), "=r"(d[31])
-            : "r"(taddr)
+            "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+            "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n\t"
+            "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+            "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n\t"
+            "tcgen05.wait::ld.sync.aligned;"
+            : "=r"(lo[0]), "=r"(lo[1]), "=r"(lo[2]), "=r"(lo[3]), "=r"(lo[4]), "=r"(lo[5]), "=r"(lo[6]), "=r"(lo[7]),
+              "=r"(lo[8]), "=r"(lo[9]), "=r"(lo[10]), "=r"(lo[11]), "=r"(lo[12]), "=r"(lo[13]), "=r"(lo[14]), "=r"(lo[15]),
+              "=r"(lo[16]), "=r"(lo[17]), "=r"(lo[18]), "=r"(lo[19]), "=r"(lo[20]), "=r"(lo[21]), "=r"(lo[22]), "=r"(lo[23]),
+              "=r"(lo[24]), "=r"(lo[25]), "=r"(lo[26]), "=r"(lo[27]), "=r"(lo[28]), "=r"(lo[29]), "=r"(lo[30]), "=r"(lo[31]),
+              "=r"(hi[0]), "=r"(hi[1]), "=r"(hi[2]), "=r"(hi[3]), "=r"(hi[4]), "=r"(hi[5]), "=r"(hi[6]), "=r"(hi[7]),
+              "=r"(hi[8]), "=r"(hi[9]), "=r"(hi[10]), "=r"(hi[11]), "=r"(hi[12]), "=r"(hi[13]), "=r"(hi[14]), "=r"(hi[15]),
+              "=r"(hi[16]), "=r"(hi[17]), "=r"(hi[18]), "=r"(hi[19]), "=r"(hi[20]), "=r"(hi[21]), "=r"(hi[22]), "=r"(hi[23]),
+              "=r"(hi[24]), "=r"(hi[25]), "=r"(hi[26]), "=r"(hi[27]), "=r"(hi[28]), "=r"(hi[29]), "=r"(hi[30]), "=r"(hi[31])
+            : "r"(taddr), "r"(taddr + (16u << 16))
             : "memory");
     } else if constexpr (kCols == 32) {
         asm volatile(
-            "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7]), "=r"(d[8]), "=r"(d[9]), "=r"(d[10]), "=r"(d[11]),
-              "=r"(d[12]), "=r"(d[13]), "=r"(d[14]), "=r"(d[15])
-            : "r"(taddr)
+            "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n\t"
+            "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n\t"
+            "tcgen05.wait::ld.sync.aligned;"
+            : "=r"(lo[0]), "=r"(lo[1]), "=r"(lo[2]), "=r"(lo[3]), "=r"(lo[4]), "=r"(lo[5]), "=r"(lo[6]), "=r"(lo[7]),
+              "=r"(lo[8]), "=r"(lo[9]), "=r"(lo[10]), "=r"(lo[11]), "=r"(lo[12]), "=r"(lo[13]), "=r"(lo[14]), "=r"(lo[15]),
+              "=r"(hi[0]), "=r"(hi[1]), "=r"(hi[2]), "=r"(hi[3]), "=r"(hi[4]), "=r"(hi[5]), "=r"(hi[6]), "=r"(hi[7]),
+              "=r"(hi[8]), "=r"(hi[9]), "=r"(hi[10]), "=r"(hi[11]), "=r"(hi[12]), "=r"(hi[13]), "=r"(hi[14]), "=r"(hi[15])
+            : "r"(taddr), "r"(taddr + (16u << 16))
             : "memory");
     } else {
-        asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7])
-                     : "r"(taddr)
-                     : "memory");
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%16];\n\t"
+            "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%17];\n\t"
+            "tcgen05.wait::ld.sync.aligned;"
+            : "=r"(lo[0]), "=r"(lo[1]), "=r"(lo[2]), "=r"(lo[3]), "=r"(lo[4]), "=r"(lo[5]), "=r"(lo[6]), "=r"(lo[7]),
+              "=r"(hi[0]), "=r"(hi[1]), "=r"(hi[2]), "=r"(hi[3]), "=r"(hi[4]), "=r"(hi[5]), "=r"(hi[6]), "=r"(hi[7])
+            : "r"(taddr), "r"(taddr + (16u << 16))
+            : "memory");
     }
 }
 // where head h's weight stands in its row, so that a thread's are 16 bytes at a time: 16 j + 4 (t % 4) + ..
@@ -371,28 +393,46 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
         uint32_t exchanges = 0;
         bool ok = true;
         int done = 0;      // items
-        // A score to its place: s of position pos, -inf unless it counts; `stored`: the row is one.
+        // A score to its place: s of position pos, -inf unless it counts; `stored`: the row is one.  Blocks of more than a warp's positions are joined
+        // over the warpgroup when the next row's scores are there (or the item ends), by when the other warps' parts have long come (joined
+        // at once, 1500 rows of 32 heads in blocks of 64 took 103 instead of 83 us).
+        bool pending = false, pending_stored = false;
+        float pending_s = 0.0f;
+        float* pending_at = nullptr;
+        auto join = [&]() {
+            if (!pending) return;
+            pending = false;
+            const int buf = (exchanges - 1) & 1;   // (a third job's value is written after the exchange of the second)
+            ok = ok && wait(bar_at(offsetof(Control, exchange), wg), buf, abort_flag);
+            float s = max_nan(pending_s, ctl->best[wg][buf][sub ^ 1]);
+            if (block == 128) s = max_nan(s, max_nan(ctl->best[wg][buf][sub ^ 2], ctl->best[wg][buf][sub ^ 3]));
+            if (pending_stored) *pending_at = s;
+        };
         auto put = [&](float s, bool counts, int pos, float* at, bool stored) {
             s = counts ? s : -INFINITY;
+            stored = stored && pos < kv_len;
             if (block == 1) {
-                if (stored && pos < kv_len) *at = s;
+                if (stored) *at = s;
                 return;
             }
-            for (int off = 1; off < min(block, 32); off <<= 1) s = max_nan(s, __shfl_xor_sync(0xffffffffu, s, lane_of_offset(off)));
-            if (block >= 64) {
-                const int buf = exchanges & 1;   // (a third job's value is written after the exchange of the second)
-                const uint32_t bar = bar_at(offsetof(Control, exchange), wg);
-                __syncwarp();
-                if (lane == 0) {
-                    ctl->best[wg][buf][sub] = s;
-                    mbar_arrive(bar);
-                }
-                ok = ok && wait(bar, buf, abort_flag);
-                ++exchanges;
-                s = max_nan(s, ctl->best[wg][buf][sub ^ 1]);
-                if (block == 128) s = max_nan(s, max_nan(ctl->best[wg][buf][sub ^ 2], ctl->best[wg][buf][sub ^ 3]));
+            stored = stored && (pos & (block - 1)) == 0;
+            if (block < 32) {
+                for (int off = 1; off < block; off <<= 1) s = max_nan(s, __shfl_xor_sync(0xffffffffu, s, lane_of_offset(off)));
+            } else {
+                s = warp_max_nan(s);
             }
-            if ((pos & (block - 1)) == 0 && stored && pos < kv_len) *at = s;
+            if (block < 64) {
+                if (stored) *at = s;
+                return;
+            }
+            join();
+            __syncwarp();
+            if (lane == 0) {
+                ctl->best[wg][exchanges & 1][sub] = s;
+                mbar_arrive(bar_at(offsetof(Control, exchange), wg));
+            }
+            ++exchanges;
+            pending = true, pending_stored = stored, pending_s = s, pending_at = at;
         };
         // (acc_full has an arrival of the MMA warp's own besides the MMAs': what that warp saw in the tile's barrier is visible here)
         auto tile_facts = [&](float& ks, bool& here) {
@@ -402,10 +442,6 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
             if (lane == 0) mbar_arrive(bar_at(offsetof(Control, k_empty), k.s));
         };
         uint32_t lo[kCols / 2], hi[kCols / 2];
-        auto load_row = [&](uint32_t at) {
-            load_half<kCols>(at, lo);
-            load_half<kCols>(at + (16u << 16), hi);
-        };
         auto give_back = [&](uint32_t bar) {
             tc_fence_before();
             __syncwarp();
@@ -427,22 +463,22 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
                 for (int i = 0; i < it.tiles; ++i, pos += kTile, out += step) {
                     if (!(ok = ok && wait(full, acc.ph, abort_flag))) break;
                     tc_fence_after();
-                    load_row(at);
+                    load_row<kCols>(at, lo, hi);
                     float ks;
                     bool here;
                     tile_facts(ks, here);
                     float* o = out;
 #pragma unroll
                     for (int j = 0; j < kRows; ++j, o += stride) {
-                        tmem_wait_ld();
                         if (j == kRows - 1) give_back(empty);
                         const float s = sum_heads<kFp8, kCols, kAll>(lo, hi, w + j * kCols * 4, p.H, lane) * ks;
-                        if (j + 1 < kRows) load_row(at + (j + 1) * kCols);
+                        if (j + 1 < kRows) load_row<kCols>(at + (j + 1) * kCols, lo, hi);
                         put(s, here && pos < end[j], pos, o, end[j] >= 0);
                     }
                     acc.ph ^= 1u;
                     k.next(p.stages);
                 }
+                join();
                 if (!ok) break;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_at(offsetof(Control, w_empty), wb.s));
@@ -461,19 +497,19 @@ __global__ void __launch_bounds__(32 * kWarps, 1) index_scores_kernel(const __gr
                     if (!(ok = wait(bar_at(offsetof(Control, acc_full), fl.s), fl.ph, abort_flag))) break;
                     tc_fence_after();
                     uint32_t at = lanes + acc.s * p.acc_cols, w = base + p.off_w + wb.s * p.per * kCols * 4 + 16 * (lane & 3);
-                    load_row(at);
+                    load_row<kCols>(at, lo, hi);
                     float ks;
                     bool here;
                     tile_facts(ks, here);
                     float* out = p.out + (int64_t)it.q0 * p.stride_o_row + (pos >> p.block_shift);
                     for (int r = 0; r < it.rows; ++r, w += kCols * 4, out += p.stride_o_row) {
-                        tmem_wait_ld();
                         if (r == it.rows - 1) give_back(bar_at(offsetof(Control, acc_empty), acc.s));
                         const float s = sum_heads<kFp8, kCols, kAll>(lo, hi, w, p.H, lane) * ks;
-                        if (r + 1 < it.rows) load_row(at += kCols);
+                        if (r + 1 < it.rows) load_row<kCols>(at += kCols, lo, hi);
                         put(s, here && pos < ctl->valid[wb.s][r], pos, out, true);
                     }
                 }
+                join();
                 if (!ok) break;
                 turn = i - it.tiles;
                 __syncwarp();

@@ -77,6 +77,18 @@ def test_scores_of_several_rows_are_those_of_each(built_lib, fp8, s_q, H):
         assert torch.equal(api.index_scores(kv_len=kv_len, s_q=s_q, **x), whole)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("H,block", [(64, 1), (64, 64), (32, 1), (16, 128), (24, 32)])
+def test_scores_of_a_chunk_are_those_of_its_rows(built_lib, fp8, H, block):
+    """Full tiles of query rows on every SM, time and again, against one row a tile (the rows as sequences of one shared cache)."""
+    T, kv_len = 2048, 8192
+    x = problem(1, T, H, kv_len, fp8, seed=H)
+    x.pop("block_table")
+    alone = api.index_scores(kv_len=kv_len, block=block, **x)
+    for _ in range(10):
+        assert torch.equal(api.index_scores(kv_len=kv_len, s_q=T, block=block, **x), alone)
+
+
 def test_calls_on_two_streams_at_once(built_lib):
     """Every operator on two side streams at the same time gives the bits that it gives alone."""
     xs = [problem(4, 2, 64, 20000, True, seed=s) for s in (1, 2)]
