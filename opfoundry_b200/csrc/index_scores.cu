@@ -7,8 +7,12 @@
 //
 // Roles of a CTA (one an SM): warps 0-15 take the scores out of TMEM (four warpgroups, a query row at a time each), warp 16 brings tiles
 // of 128 keys page by page (TMA; an fp8 cache's scales by bulk copies), warp 17 the query rows, their weights and lengths, warp 18
-// issues the MMAs.  A work item is a group of query rows of one sequence and a chunk of tiles; the CTAs take items in turn, so the
-// ends of short rows (whose columns are only filled) are spread over them.
+// issues the MMAs.  A work item is tiles of a group of query rows of one sequence.  The tiles that the rows see are dealt out evenly over the CTAs
+// (up to 1024 groups; more take chunks in turn: 64 sequences of 16384 to 32768 positions x 2 rows took 66 instead of 47 us that way), and columns
+// that no row sees are filled by warps that have nothing else to do.
+//
+// Bounds: decode HBM (fp8: 64 x 2 rows, 53 us for 208 MB), long chunks the power cap (4096 rows over 16384 positions: 515 us in a short run, 590 in a
+// long one at 1.72 GHz; bf16 637 and 745), where the MMAs take two fifths of the cycles and the sums over heads two thirds of the issue slots.
 #include <cuda_bf16.h>
 #include <cstddef>
 #include <mutex>
@@ -280,8 +284,8 @@ __device__ __forceinline__ int lane_position(int lane) { return (lane >> 2) + 8 
 __device__ __forceinline__ int lane_of_offset(int off) { return off < 8 ? 4 * off : off >> 3; }
 
 // The sum of w_h max(0, d_h) over a pair of heads is two maxima (half rate) and two multiply-adds.  With max(0, d) taken as (d + |d|) / 2 it is a
-// two-wide multiply-add and two with |d|, three instructions: 533 instead of 540 us for 4096 rows over 16384 positions, and 71.7 instead of 69.1
-// for 64 x 2 rows over 32768, so it stays out.
+// two-wide multiply-add and two with |d|, three instructions: within 1 % for 4096 rows over 16384 positions (510 to 512 us) and slower for 64 x 2 rows
+// over 32768 (71.7 instead of 69.1), so it stays out.
 struct Sum {
     float a = 0.0f, b = 0.0f;
     __device__ __forceinline__ void add(uint32_t d0, uint32_t d1, float u, float v) {

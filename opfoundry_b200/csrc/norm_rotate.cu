@@ -2,7 +2,9 @@
 //
 // A vector x of one head (or one latent): with mu its mean (0 unless centred), y = (x - mu) / sqrt(mean((x - mu)^2) + eps) * w + b, then
 // pairs of its rotated values turned by the angle of the token's position, then one rounding to bf16, or to e4m3 with scale = amax / 448.
-// Everything between the load and that rounding is fp32.  Bound by HBM: every value is read and written once.
+// Everything between the load and that rounding is fp32.  Bound by HBM: every value is read and written once (4091 tokens of 64 + 8 heads of 128 in
+// 31 us, 4.9 TB/s); a few tokens by the launch (1.7 us in a graph), and appends by their chain position -> page -> row (64 tokens 2.4 us, 16384 into the
+// fp8 caches 12.5).
 #include <cuda_bf16.h>
 #include <type_traits>
 #include "front.h"
