@@ -107,7 +107,7 @@ template <int kHeads> __device__ __forceinline__ RotateUnit unit_of(const Rotate
 // stay zeros.
 template <int kLanes> __device__ __forceinline__ float centred_rstd(float (&v)[8], bool inside, float inv_dim, bool center, float eps) {
     if (center) {
-        const float mean = sum_over<kLanes>(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]))) * inv_dim;
+        const float mean = __fmul_rn(sum_over<kLanes>(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]))), inv_dim);
         if (inside)
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] -= mean;
@@ -120,6 +120,11 @@ template <int kLanes> __device__ __forceinline__ float centred_rstd(float (&v)[8
     }
     return rsqrtf(fmaf(sum_over<kLanes>(t + u), inv_dim, eps));
 }
+// A pair turned.  Products and sums of rotation, norm and shift are written out, so that a token's bytes are the same in every variant (left to the
+// compiler, each variant fuses another product).
+__device__ __forceinline__ float turned0(float a, float e, float co, float si) { return __fmaf_rn(-e, si, __fmul_rn(a, co)); }
+__device__ __forceinline__ float turned1(float a, float e, float co, float si) { return __fmaf_rn(e, co, __fmul_rn(a, si)); }
+__device__ __forceinline__ float scaled(float y, float rstd, float w) { return __fmul_rn(__fmul_rn(y, rstd), w); }
 __device__ __forceinline__ void store8(__nv_bfloat16* out, const float (&v)[8]) {
     *reinterpret_cast<uint4*>(out) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
@@ -273,14 +278,14 @@ __global__ void __launch_bounds__(kRotateThreads, kHeads == 1 || sizeof(In) == 2
             const float rstd = centred_rstd<kLanes>(y, inside, p.inv_dim, center, p.eps);   // (the whole warp, whichever side its heads are of)
             if (norm) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = y[i] * rstd * w[i];
+                for (int i = 0; i < 8; ++i) y[i] = scaled(y[i], rstd, w[i]);
                 if (shifted) {
                     float b[8];
                     Raw<float, kPairs> t;
                     t.load(s.bias + c0, apart, inside);
                     t.get(b);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) y[i] += b[i];
+                    for (int i = 0; i < 8; ++i) y[i] = __fadd_rn(y[i], b[i]);
                 }
             }
         }
@@ -289,8 +294,8 @@ __global__ void __launch_bounds__(kRotateThreads, kHeads == 1 || sizeof(In) == 2
             for (int i = 0; i < 4; ++i) {
                 const int i0 = kPairs ? 2 * i : i, i1 = kPairs ? 2 * i + 1 : i + 4;
                 const float a = y[i0], e = y[i1];
-                y[i0] = a * co[i] - e * si[i];
-                y[i1] = a * si[i] + e * co[i];
+                y[i0] = turned0(a, e, co[i], si[i]);
+                y[i1] = turned1(a, e, co[i], si[i]);
             }
         if constexpr (kE4m3) {
             float amax = 0.0f;
@@ -347,7 +352,7 @@ __global__ void __launch_bounds__(256) norm_rotate_long_kernel(const __grid_cons
             for (int k = 0; k < kVecs; ++k)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) t += v[k][i];
-            mean = sum_over<32>(t) * p.inv_dim;
+            mean = __fmul_rn(sum_over<32>(t), p.inv_dim);
         }
         float t = 0.0f;
 #pragma unroll
@@ -363,7 +368,10 @@ __global__ void __launch_bounds__(256) norm_rotate_long_kernel(const __grid_cons
         load8(s.weight + c, w);
         if (s.bias != nullptr) load8(s.bias + c, b);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = (y[i] - mean) * rstd * w[i] + (s.bias != nullptr ? b[i] : 0.0f);
+        for (int i = 0; i < 8; ++i) y[i] = scaled(__fsub_rn(y[i], mean), rstd, w[i]);
+        if (s.bias != nullptr)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = __fadd_rn(y[i], b[i]);
     };
     const float* table = p.cos_sin + (int64_t)u.pos * p.rope_dim;
     const int half = p.rope_dim / 2;
@@ -381,8 +389,8 @@ __global__ void __launch_bounds__(256) norm_rotate_long_kernel(const __grid_cons
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float a = v[k][2 * i], b = v[k][2 * i + 1];
-                v[k][2 * i] = a * co[i] - b * si[i];
-                v[k][2 * i + 1] = a * si[i] + b * co[i];
+                v[k][2 * i] = turned0(a, b, co[i], si[i]);
+                v[k][2 * i + 1] = turned1(a, b, co[i], si[i]);
             }
         } else {
             const bool upper = r >= half;
@@ -392,7 +400,7 @@ __global__ void __launch_bounds__(256) norm_rotate_long_kernel(const __grid_cons
             load8(table + r - (upper ? half : 0), co);
             load8(table + half + r - (upper ? half : 0), si);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[k][i] = upper ? o[i] * si[i] + v[k][i] * co[i] : v[k][i] * co[i] - o[i] * si[i];
+            for (int i = 0; i < 8; ++i) v[k][i] = upper ? turned1(o[i], v[k][i], co[i], si[i]) : turned0(v[k][i], o[i], co[i], si[i]);
         }
     }
     if constexpr (kE4m3) {
@@ -552,11 +560,11 @@ template <typename In, bool kFp8, int kTokens> __device__ __forceinline__ void a
         if (row[k] < 0) continue;
         uint32_t rope;
         if (pairs) {
-            rope = pack_bf16x2(pe[k][0] * co[k][0] - pe[k][1] * si[k][0], pe[k][0] * si[k][0] + pe[k][1] * co[k][0]);
+            rope = pack_bf16x2(turned0(pe[k][0], pe[k][1], co[k][0], si[k][0]), turned1(pe[k][0], pe[k][1], co[k][0], si[k][0]));
         } else {
             const float o0 = __shfl_xor_sync(0xffffffffu, pe[k][0], 16), o1 = __shfl_xor_sync(0xffffffffu, pe[k][1], 16);
-            rope = lane >= 16 ? pack_bf16x2(o0 * si[k][0] + pe[k][0] * co[k][0], o1 * si[k][1] + pe[k][1] * co[k][1])
-                              : pack_bf16x2(pe[k][0] * co[k][0] - o0 * si[k][0], pe[k][1] * co[k][1] - o1 * si[k][1]);
+            rope = lane >= 16 ? pack_bf16x2(turned1(o0, pe[k][0], co[k][0], si[k][0]), turned1(o1, pe[k][1], co[k][1], si[k][1]))
+                              : pack_bf16x2(turned0(pe[k][0], o0, co[k][0], si[k][0]), turned0(pe[k][1], o1, co[k][1], si[k][1]));
         }
         uint64_t v[8];
 #pragma unroll
@@ -649,16 +657,16 @@ template <typename In, bool kFp8, int kTokens> __device__ __forceinline__ void a
         if (norm) {
             const float rstd = centred_rstd<16>(y, true, 1.0f / kDIndex, p.a.index_center, p.a.eps);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = y[i] * rstd * w[i];
+            for (int i = 0; i < 8; ++i) y[i] = scaled(y[i], rstd, w[i]);
             if (shifted)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] += b[i];
+                for (int i = 0; i < 8; ++i) y[i] = __fadd_rn(y[i], b[i]);
         }
         if (turns && row[k] >= 0) {
             auto turn = [&](float& a, float& e, int i) {
                 const float x = a;
-                a = x * co[k][i] - e * si[k][i];
-                e = x * si[k][i] + e * co[k][i];
+                a = turned0(x, e, co[k][i], si[k][i]);
+                e = turned1(x, e, co[k][i], si[k][i]);
             };
             if (pairs) {
 #pragma unroll

@@ -89,6 +89,39 @@ def test_scores_of_a_chunk_are_those_of_its_rows(built_lib, fp8, H, block):
         assert torch.equal(api.index_scores(kv_len=kv_len, s_q=T, block=block, **x), alone)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_many_tokens_are_those_of_few(built_lib, fp8, dtype, interleaved):
+    """5003 tokens in one call, where a warp takes several tokens or heads, give the bits of calls of 100; every seventh is padding."""
+    g = gen(9)
+    T, H, Hk, P = 5003, 9, 2, 6000
+    pages = -(-P // 64)
+    rt, pos = rope_table(64, P).cuda(), torch.randperm(P, generator=g)[:T].to(torch.int32)
+    pos[::7] = -1
+    pos = pos.cuda()
+    table = torch.randperm(pages, generator=g)[None].to(torch.int32).cuda()
+    x, key, q, k = (torch.randn(T, *s, generator=g).to(dtype).cuda() for s in ((576,), (128,), (H, 128), (Hk, 128)))
+    w, iw, ib = (1 + 0.1 * torch.randn(n, generator=g).cuda() for n in (512, 128, 128))
+    got = []
+    for step in (T, 100):
+        kv = torch.full((pages * 64, 656), 7, dtype=torch.uint8, device="cuda") if fp8 else torch.full((pages * 64, 576), 7.0, dtype=torch.bfloat16, device="cuda")
+        index = api.index_cache_pages(pages, fp8)
+        od = E4M3 if fp8 else torch.bfloat16
+        qo, ko = torch.full((T, H, 128), 7.0, device="cuda").to(od), torch.full((T, Hk, 128), 7.0, device="cuda").to(od)
+        qs, ks = (torch.full((T, n), 7.0, device="cuda") if fp8 else None for n in (H, Hk))
+        for a in range(0, T, step):
+            b = slice(a, a + step)
+            api.append_cache(x[b, :512], x[b, 512:], kv, rt, pos[b], s_q=T, block_table=table, latent_weight=w, index_key=key[b], index_cache=index, index_weight=iw,
+                             index_bias=ib, index_center=True, interleaved=interleaved)
+            api.norm_rotate(q[b], rt, pos[b], k=k[b], q_weight=iw, q_bias=ib, k_weight=iw, center=True, interleaved=interleaved, q_out=qo[b], k_out=ko[b],
+                            **(dict(q_scale=qs[b], k_scale=ks[b]) if fp8 else {}))
+        got.append([kv, index, qo.view(torch.uint8), ko.view(torch.uint8)] + ([qs, ks] if fp8 else []))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert (got[0][2].view(E4M3 if fp8 else torch.bfloat16)[::7].float() == 7).all()
+
+
 def test_calls_on_two_streams_at_once(built_lib):
     """Every operator on two side streams at the same time gives the bits that it gives alone."""
     xs = [problem(4, 2, 64, 20000, True, seed=s) for s in (1, 2)]
