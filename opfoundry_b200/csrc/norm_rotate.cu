@@ -103,12 +103,12 @@ template <int kHeads> __device__ __forceinline__ RotateUnit unit_of(const Rotate
     if (!u.live) u.count = 0;
     return u;
 }
-// Subtracts the mean (center) and returns 1 / sqrt(mean of the squares + eps) (rsqrtf: two units in the last place).  Values behind the vector
-// stay zeros.
-template <int kLanes> __device__ __forceinline__ float centred_rstd(float (&v)[8], bool inside, float inv_dim, bool center, float eps) {
+// Subtracts the mean (center) and returns 1 / sqrt(mean of the squares + eps) (rsqrtf: two units in the last place).  The whole warp takes part in
+// the sums, so `center` is the same for all of it; a lane whose vector has no norm, or that is behind its vector, keeps its values (`subtract`).
+template <int kLanes> __device__ __forceinline__ float centred_rstd(float (&v)[8], bool subtract, float inv_dim, bool center, float eps) {
     if (center) {
         const float mean = __fmul_rn(sum_over<kLanes>(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]))), inv_dim);
-        if (inside)
+        if (subtract)
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] -= mean;
     }
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kRotateThreads, kHeads == 1 || sizeof(In) == 2
     Raw<In, kPairs> raw[kHeads];
 #pragma unroll
     for (int k = 0; k < kHeads; ++k, x += x_head) raw[k].load(x, apart, k < count);
-    const bool norm = kNorm && s.weight != nullptr, center = kNorm && norm && p.center, shifted = norm && s.bias != nullptr;
+    const bool norm = kNorm && s.weight != nullptr, shifted = norm && s.bias != nullptr;
     float w[8], co[4], si[4];
     if (norm) {
         Raw<float, kPairs> t;
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kRotateThreads, kHeads == 1 || sizeof(In) == 2
         float y[8];
         raw[k].get(y);
         if (kNorm) {
-            const float rstd = centred_rstd<kLanes>(y, inside, p.inv_dim, center, p.eps);   // (the whole warp, whichever side its heads are of)
+            const float rstd = centred_rstd<kLanes>(y, inside && norm, p.inv_dim, p.center, p.eps);   // (the whole warp, whichever side its heads are of)
             if (norm) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = scaled(y[i], rstd, w[i]);
