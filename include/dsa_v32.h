@@ -438,7 +438,7 @@ typedef struct dsa_v32_append_args {
     const int32_t* seq_ids;    /* [num_tokens] or NULL */
     const int32_t* block_table;
     int64_t stride_latent, stride_rope, stride_index_key;
-    int64_t num_kv_rows;       /* rows of either cache */
+    int64_t num_kv_rows;       /* rows of either cache; with an fp8 index cache whole pages */
     int64_t kv_batch_stride_rows;
     int32_t num_tokens, s_q, num_seqs, block_table_stride, page_block_size, max_positions;
     int32_t in_dtype, kv_dtype;

@@ -926,6 +926,8 @@ int dsa_v32_append_cache(const dsa_v32_append_args* a, void* stream) {
     if (a->num_kv_rows <= 0 || a->num_kv_rows >= (int64_t(1) << 31) - 1 || a->page_block_size <= 0) return DSA_V32_ERR_SHAPE;
     if (a->block_table ? a->block_table_stride <= 0 : a->kv_batch_stride_rows < 0) return DSA_V32_ERR_SHAPE;
     if (a->index_cache && !index_page_ok(a->page_block_size)) return DSA_V32_ERR_SHAPE;
+    // scales stand behind all keys of their page, so a part of a page does not hold its rows (bf16 rows have no such place)
+    if (a->index_cache && a->kv_dtype == DSA_V32_KV_FP8 && a->num_kv_rows % a->page_block_size) return DSA_V32_ERR_SHAPE;
     if (!(a->eps >= 0.0f) || !std::isfinite(a->eps)) return DSA_V32_ERR_SHAPE;
     if (a->num_tokens == 0) return DSA_V32_OK;
     if (!a->positions || !a->cos_sin || (a->kv && (!a->latent || !a->rope)) || (a->index_cache && !a->index_key)) return DSA_V32_ERR_NULL;

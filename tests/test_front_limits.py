@@ -1,0 +1,23 @@
+"""Refusals at the borders of the front end's argument blocks, before anything is launched (no GPU)."""
+import ctypes as C
+
+import pytest
+
+from opfoundry_b200 import api
+from test_front_args import SHAPE, append_args, refused
+
+
+@pytest.mark.parametrize("rows", [650, 639, 1])
+def test_append_refuses_parts_of_fp8_index_pages(built_lib, rows):
+    """A page's scales stand behind its keys: those of a part of a page would lie behind the cache."""
+    for changes in (dict(), dict(kv=None)):
+        refused(built_lib.dsa_v32_append_cache, append_args, dict(kv_dtype=api.KV_FP8, num_kv_rows=rows) | changes, SHAPE)
+
+
+@pytest.mark.parametrize("changes", [dict(kv_dtype=api.KV_BF16, num_kv_rows=650), dict(kv_dtype=api.KV_FP8, num_kv_rows=650, index_cache=None),
+                                     dict(kv_dtype=api.KV_FP8, num_kv_rows=640)])
+def test_append_takes_rows_without_pages_of_scales(built_lib, changes):
+    a = append_args()
+    for k, v in (changes | dict(num_tokens=0)).items():
+        setattr(a, k, v)
+    assert built_lib.dsa_v32_append_cache(C.byref(a), None) == 0
