@@ -14,8 +14,13 @@ namespace dsa {
 namespace {
 
 // ------------------------------------------------------------------ values
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+// Loads through the read-only path (kReadOnly) may be moved across barriers, so vectors that may be turned in place are read without it.
+template <bool kReadOnly, typename T> __device__ __forceinline__ T load_as(const void* p) {
+    if constexpr (kReadOnly) return __ldg(reinterpret_cast<const T*>(p));
+    else return *reinterpret_cast<const T*>(p);
+}
+template <bool kReadOnly> __device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 u = load_as<kReadOnly, uint4>(p);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -23,8 +28,8 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
         v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     }
 }
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+template <bool kReadOnly> __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    const float4 a = load_as<kReadOnly, float4>(p), b = load_as<kReadOnly, float4>(p + 4);
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 __device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
@@ -176,12 +181,12 @@ __device__ __forceinline__ uint2 quotients8(const float (&v)[8], float scale) {
 __device__ __forceinline__ void put_scale(const RotateSide& s, int64_t at, float scale) { s.scale[at] = s.gate != nullptr ? scale * __ldg(s.gate + at) : scale; }
 
 // Eight values as they come: one 16-byte load of bf16, or two loads, the second `apart` values further on.
-template <typename In, bool kPairs> struct Raw;
-template <> struct Raw<__nv_bfloat16, true> {
+template <typename In, bool kPairs, bool kReadOnly> struct Raw;
+template <bool kReadOnly> struct Raw<__nv_bfloat16, true, kReadOnly> {
     uint4 u;
     __device__ __forceinline__ void load(const __nv_bfloat16* p, int64_t, bool there) {
         u = make_uint4(0u, 0u, 0u, 0u);
-        if (there) u = __ldg(reinterpret_cast<const uint4*>(p));
+        if (there) u = load_as<kReadOnly, uint4>(p);
     }
     __device__ __forceinline__ void get(float (&v)[8]) const {
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -192,13 +197,13 @@ template <> struct Raw<__nv_bfloat16, true> {
         }
     }
 };
-template <> struct Raw<__nv_bfloat16, false> {
+template <bool kReadOnly> struct Raw<__nv_bfloat16, false, kReadOnly> {
     uint2 a, b;
     __device__ __forceinline__ void load(const __nv_bfloat16* p, int64_t apart, bool there) {
         a = b = make_uint2(0u, 0u);
         if (there) {
-            a = __ldg(reinterpret_cast<const uint2*>(p));
-            b = __ldg(reinterpret_cast<const uint2*>(p + apart));
+            a = load_as<kReadOnly, uint2>(p);
+            b = load_as<kReadOnly, uint2>(p + apart);
         }
     }
     __device__ __forceinline__ void get(float (&v)[8]) const {
@@ -210,13 +215,13 @@ template <> struct Raw<__nv_bfloat16, false> {
         }
     }
 };
-template <bool kPairs> struct Raw<float, kPairs> {
+template <bool kPairs, bool kReadOnly> struct Raw<float, kPairs, kReadOnly> {
     float4 a, b;
     __device__ __forceinline__ void load(const float* p, int64_t apart, bool there) {
         a = b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (there) {
-            a = __ldg(reinterpret_cast<const float4*>(p));
-            b = __ldg(reinterpret_cast<const float4*>(p + apart));
+            a = load_as<kReadOnly, float4>(p);
+            b = load_as<kReadOnly, float4>(p + apart);
         }
     }
     __device__ __forceinline__ void get(float (&v)[8]) const { v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w; }
@@ -253,13 +258,14 @@ __global__ void __launch_bounds__(kRotateThreads, kHeads == 1 || sizeof(In) == 2
     const int64_t x_head = s.x_head, o_head = s.o_head;
     const int64_t apart = kPairs ? 4 : c1 - c0;
     const In* x = reinterpret_cast<const In*>(s.x) + u.token * s.x_row + u.head * x_head + c0;
-    Raw<In, kPairs> raw[kHeads];
+    constexpr bool kApart = kE4m3 || sizeof(In) != 2;   // the output's type is another one, so it is not the input
+    Raw<In, kPairs, kApart> raw[kHeads];
 #pragma unroll
     for (int k = 0; k < kHeads; ++k, x += x_head) raw[k].load(x, apart, k < count);
     const bool norm = kNorm && s.weight != nullptr, shifted = norm && s.bias != nullptr;
     float w[8], co[4], si[4];
     if (norm) {
-        Raw<float, kPairs> t;
+        Raw<float, kPairs, true> t;
         t.load(s.weight + c0, apart, inside);         // (lanes behind the vector stay zero)
         t.get(w);
     }
@@ -281,7 +287,7 @@ __global__ void __launch_bounds__(kRotateThreads, kHeads == 1 || sizeof(In) == 2
                 for (int i = 0; i < 8; ++i) y[i] = scaled(y[i], rstd, w[i]);
                 if (shifted) {
                     float b[8];
-                    Raw<float, kPairs> t;
+                    Raw<float, kPairs, true> t;
                     t.load(s.bias + c0, apart, inside);
                     t.get(b);
 #pragma unroll
@@ -327,6 +333,7 @@ __global__ void __launch_bounds__(kRotateThreads, kHeads == 1 || sizeof(In) == 2
 template <typename In, bool kE4m3, int kVecs>
 __global__ void __launch_bounds__(256) norm_rotate_long_kernel(const __grid_constant__ RotateParams p) {
     grid_dependency_wait();
+    constexpr bool kApart = kE4m3 || sizeof(In) != 2;   // the output's type is another one, so it is not the input
     const int lane = threadIdx.x & 31;
     const RotateUnit u = unit_of<1>(p, (int64_t)blockIdx.x * 8 + threadIdx.x / 32);
     const RotateSide& s = p.side[u.is_q ? 0 : 1];
@@ -337,7 +344,7 @@ __global__ void __launch_bounds__(256) norm_rotate_long_kernel(const __grid_cons
     for (int k = 0; k < kVecs; ++k) {
         const int c = 8 * (lane + k * 32);
         if (c < p.head_dim) {
-            load8(x + c, v[k]);
+            load8<kApart>(x + c, v[k]);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[k][i] = 0.0f;
@@ -365,8 +372,8 @@ __global__ void __launch_bounds__(256) norm_rotate_long_kernel(const __grid_cons
     auto normed = [&](float (&y)[8], int c) {
         if (!norm) return;
         float w[8], b[8];
-        load8(s.weight + c, w);
-        if (s.bias != nullptr) load8(s.bias + c, b);
+        load8<true>(s.weight + c, w);
+        if (s.bias != nullptr) load8<true>(s.bias + c, b);
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = scaled(__fsub_rn(y[i], mean), rstd, w[i]);
         if (s.bias != nullptr)
@@ -395,10 +402,10 @@ __global__ void __launch_bounds__(256) norm_rotate_long_kernel(const __grid_cons
         } else {
             const bool upper = r >= half;
             float o[8], co[8], si[8];
-            load8(x + c + (upper ? -half : half), o);
+            load8<kApart>(x + c + (upper ? -half : half), o);
             normed(o, c + (upper ? -half : half));
-            load8(table + r - (upper ? half : 0), co);
-            load8(table + half + r - (upper ? half : 0), si);
+            load8<true>(table + r - (upper ? half : 0), co);
+            load8<true>(table + half + r - (upper ? half : 0), si);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[k][i] = upper ? turned1(o[i], v[k][i], co[i], si[i]) : turned0(v[k][i], o[i], co[i], si[i]);
         }
@@ -418,7 +425,7 @@ __global__ void __launch_bounds__(256) norm_rotate_long_kernel(const __grid_cons
         }
         if (lane == 0) put_scale(s, u.token * (u.is_q ? p.q_heads : p.heads - p.q_heads) + u.head, scale);
     } else {
-        __syncwarp();   // in place: a lane's values may still be another's partners
+        if constexpr (!kApart) __syncwarp();   // in place: a lane's values may still be another's partners
         __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(s.out) + u.token * s.o_row + u.head * s.o_head;
 #pragma unroll
         for (int k = 0; k < kVecs; ++k) {
@@ -517,7 +524,7 @@ template <int kTokens> __device__ __forceinline__ Placed place(const AppendParam
 // kTokens tokens are loaded before their places are known.
 template <typename In, bool kFp8, int kTokens> __device__ __forceinline__ void append_latents(const AppendParams& p, int first, int lane) {
     const int n = p.a.num_tokens;
-    Raw<In, true> raw[kTokens][2];
+    Raw<In, true, true> raw[kTokens][2];
     float pe[kTokens][2];
 #pragma unroll
     for (int k = 0; k < kTokens; ++k) {
@@ -623,7 +630,7 @@ template <typename In, bool kFp8, int kTokens> __device__ __forceinline__ void a
     const int n = p.a.num_tokens, l = lane & 15, mine = lane >> 4;
     const bool pairs = p.a.index_interleaved, turns = l < 8;
     const int c0 = pairs || !turns ? 8 * l : 4 * l, apart = pairs || !turns ? 4 : 32;
-    Raw<In, false> raw[kEach];
+    Raw<In, false, true> raw[kEach];
 #pragma unroll
     for (int k = 0; k < kEach; ++k)
         raw[k].load(reinterpret_cast<const In*>(p.a.index_key) + min(first + 2 * k + mine, n - 1) * p.a.stride_index_key + c0, apart, true);
@@ -631,7 +638,7 @@ template <typename In, bool kFp8, int kTokens> __device__ __forceinline__ void a
     const bool norm = p.a.index_weight != nullptr, shifted = p.a.index_bias != nullptr;
     float w[8], b[8];
     if (norm) {
-        Raw<float, false> t;
+        Raw<float, false, true> t;
         t.load(p.a.index_weight + c0, apart, true);
         t.get(w);
         if (shifted) {
