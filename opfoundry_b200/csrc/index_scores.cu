@@ -94,9 +94,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN where eith
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
-__device__ __forceinline__ float warp_max_nan(float a) {
+__device__ __forceinline__ float warp_max_nan(float a) {   // (volatile: the whole warp executes it, also where one lane uses the result)
     float d;
-    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(a));
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(a));
     return d;
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
