@@ -982,10 +982,11 @@ int dsa_v32_index_scores(const dsa_v32_index_scores_args* a, void* stream) {
 
 int dsa_v32_block_select(const float* scores, int64_t stride_row, const int32_t* valid_len, int32_t total_q, int32_t num_blocks, int32_t block,
                          int32_t num_selected, int32_t first, int32_t local, int32_t* indices_out, void* stream) {
-    if (!scores || !indices_out) return DSA_V32_ERR_NULL;
     if (total_q < 0 || num_blocks <= 0 || block <= 0 || num_selected <= 0 || stride_row < num_blocks) return DSA_V32_ERR_SHAPE;
     if (first < 0 || local < 0 || first > num_selected - local) return DSA_V32_ERR_SHAPE;
     if ((int64_t)num_blocks * block >= (int64_t(1) << 31) || (int64_t)num_selected * block >= (int64_t(1) << 31)) return DSA_V32_ERR_SHAPE;
+    if (total_q == 0) return DSA_V32_OK;   // (empty tensors have no address)
+    if (!scores || !indices_out) return DSA_V32_ERR_NULL;
     cudaError_t e = launch_block_select(scores, stride_row, valid_len, total_q, num_blocks, block, num_selected, first, local, indices_out, (cudaStream_t)stream);
     return e == cudaSuccess ? DSA_V32_OK : (int)e;
 }

@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 
 from opfoundry_b200 import api
-from test_front_args import SHAPE, append_args, refused
+from test_front_args import BASE, NULL, SHAPE, append_args, refused
 
 
 @pytest.mark.parametrize("rows", [650, 639, 1])
@@ -21,3 +21,11 @@ def test_append_takes_rows_without_pages_of_scales(built_lib, changes):
     for k, v in (changes | dict(num_tokens=0)).items():
         setattr(a, k, v)
     assert built_lib.dsa_v32_append_cache(C.byref(a), None) == 0
+
+
+def test_block_select_of_no_rows(built_lib):
+    """Empty tensors have the address 0; shapes are checked all the same."""
+    assert built_lib.dsa_v32_block_select(None, 10, None, 0, 10, 64, 4, 0, 0, None, None) == 0
+    assert built_lib.dsa_v32_block_select(None, 10, None, 0, 10, 64, 4, 3, 2, None, None) == SHAPE
+    for scores, out in ((None, BASE), (BASE, None)):
+        assert built_lib.dsa_v32_block_select(scores, 10, None, 1, 10, 64, 4, 0, 0, out, None) == NULL
