@@ -856,8 +856,9 @@ int dsa_v32_debug_rows(const dsa_v32_attn_args* a, int32_t* rows_out, void* stre
 
 int dsa_v32_topk_select(const float* scores, int64_t stride_row, const int32_t* valid_len, int32_t total_q, int32_t kv_len,
                         int32_t topk, int32_t* indices_out, void* stream) {
-    if (!scores || !indices_out) return DSA_V32_ERR_NULL;
     if (total_q < 0 || kv_len <= 0 || topk <= 0 || stride_row < kv_len) return DSA_V32_ERR_SHAPE;
+    if (total_q == 0) return DSA_V32_OK;   // (empty tensors have no address)
+    if (!scores || !indices_out) return DSA_V32_ERR_NULL;
     cudaError_t e = launch_topk_select(scores, stride_row, valid_len, total_q, kv_len, topk, indices_out, (cudaStream_t)stream);
     return e == cudaSuccess ? DSA_V32_OK : (int)e;
 }

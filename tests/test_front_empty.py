@@ -23,3 +23,9 @@ def test_an_empty_step(built_lib, fp8):
     idx = api.block_select(s, 2, 64, pos)
     assert q8.shape == k8.shape == (0, 4, 128) and s.shape == (0, 2) and idx.shape == (0, 128)
     assert (kv == 3).all() and (index == 0).all()
+
+
+def test_an_empty_step_of_single_positions(built_lib):
+    q, pos = torch.empty(0, 4, 128, dtype=torch.bfloat16, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda")
+    s = api.index_scores(q, torch.empty(0, 4, device="cuda"), api.index_cache_pages(2, False), pos, 128)
+    assert s.shape == (0, 128) and api.topk_select(s, 16, pos).shape == (0, 16)

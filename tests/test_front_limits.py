@@ -29,3 +29,11 @@ def test_block_select_of_no_rows(built_lib):
     assert built_lib.dsa_v32_block_select(None, 10, None, 0, 10, 64, 4, 3, 2, None, None) == SHAPE
     for scores, out in ((None, BASE), (BASE, None)):
         assert built_lib.dsa_v32_block_select(scores, 10, None, 1, 10, 64, 4, 0, 0, out, None) == NULL
+
+
+def test_topk_select_of_no_rows(built_lib):
+    """The lists of single positions, from the same scores."""
+    assert built_lib.dsa_v32_topk_select(None, 10, None, 0, 10, 4, None, None) == 0
+    assert built_lib.dsa_v32_topk_select(None, 9, None, 0, 10, 4, None, None) == SHAPE
+    for scores, out in ((None, BASE), (BASE, None)):
+        assert built_lib.dsa_v32_topk_select(scores, 10, None, 1, 10, 4, out, None) == NULL
