@@ -371,7 +371,8 @@ int dsa_v32_pack_fp8_rows(const float* latent, const void* rope_bf16, const int6
  * becomes (a cos - b sin, a sin + b cos); pair i of a vector's rope_dim values is (2 i, 2 i + 1) when `interleaved`, else
  * (i, i + rope_dim / 2).  A token whose position lies outside [0, max_positions) is a padding token: nothing is written for it.
  * Norms are taken in fp32 over a whole vector: with `center` its mean is subtracted first, then x / sqrt(mean(x^2) + eps) *
- * weight + bias; a NULL weight means no norm (and no centring), a NULL bias none.  Values are rounded once, at the end.
+ * weight + bias; a NULL weight means no norm (so no centring) of those vectors, a NULL bias none.  A bias without its weight, and
+ * `center` where nothing has a weight, are refused.  Values are rounded once, at the end.
  * e4m3 outputs: scale = amax / 448 (1 for a vector of zeros), value = e4m3(x / scale), as in dsa_v32_pack_fp8_rows.
  */
 #define DSA_V32_DTYPE_BF16 0

@@ -433,8 +433,8 @@ def _vec(t, n, dtype=_F32):
 
 def norm_rotate(q, cos_sin, positions, *, k=None, q_weight=None, k_weight=None, q_bias=None, k_bias=None, center=False, eps=1e-6, rope_begin=0,
                 interleaved=True, head_weight=None, out_dtype=torch.bfloat16, q_out=None, k_out=None, q_scale=None, k_scale=None):
-    """Norm (with a weight; `center`: of the values less their mean) and rotation of every head of q [tokens, heads, dim] and, in the
-    same launch, k; bf16 or fp32 in, bf16 or float8_e4m3fn out.
+    """Norm (with a weight; `center`: of the values less their mean, refused where neither side has a weight) and rotation of every head
+    of q [tokens, heads, dim] and, in the same launch, k; bf16 or fp32 in, bf16 or float8_e4m3fn out.
 
     cos_sin fp32 [positions, rope_dim]: rope_dim / 2 cosines, then as many sines; None: no rotation.  The rope_dim values from rope_begin
     on are rotated in pairs (2 i, 2 i + 1), or (i, i + rope_dim / 2) when not `interleaved`.  positions int32 [tokens]: nothing is written for
@@ -515,8 +515,8 @@ def append_cache(latent, rope, kv, cos_sin, positions, *, seq_ids=None, s_q=1, b
                  latent_weight=None, index_key=None, index_cache=None, index_weight=None, index_bias=None, index_center=False, eps=1e-6,
                  interleaved=True, index_interleaved=None):
     """Appends tokens to the paged caches in one launch: latent [tokens, 512] (RMS norm when latent_weight is given) and rope [tokens, 64]
-    (rotated) to rows of kv (bf16 [rows, 576] or uint8 [rows, 656]), index_key [tokens, 128] (norm when index_weight is given, its first 64
-    values rotated) to index_cache of the same type (index_cache_pages).  bf16 or fp32 in.  Token t is position positions[t] of sequence
+    (rotated) to rows of kv (bf16 [rows, 576] or uint8 [rows, 656]), index_key [tokens, 128] (norm when index_weight is given, which index_center needs; its
+    first 64 values rotated) to index_cache of the same type (index_cache_pages).  bf16 or fp32 in.  Token t is position positions[t] of sequence
     seq_ids[t] (None: t // s_q); a negative sequence, a position outside cos_sin [positions, 64] or a row outside the cache writes nothing.
     latent = rope = kv = None: the index cache alone."""
     tokens = positions.shape[0]

@@ -902,6 +902,7 @@ int dsa_v32_norm_rotate(const dsa_v32_norm_rotate_args* a, void* stream) {
     if (a->rope_dim > 0 && (!a->cos_sin || !a->positions)) return DSA_V32_ERR_NULL;
     if (e4m3 && (!a->q_scale || (a->k_heads > 0 && !a->k_scale))) return DSA_V32_ERR_NULL;
     if (!e4m3 && a->head_weight) return DSA_V32_ERR_DTYPE;
+    if (a->center && !a->q_weight && !(a->k_heads > 0 && a->k_weight)) return DSA_V32_ERR_NULL;   // there is no norm that it belongs to
     const int64_t in_unit = a->in_dtype == DSA_V32_DTYPE_FP32 ? 4 : 8, d = a->head_dim;
     struct Side { const void *x, *out; const float *w, *b; int64_t row, head, o_row, o_head, heads; };
     const Side sides[2] = {{a->q, a->q_out, a->q_weight, a->q_bias, a->stride_q_row, a->stride_q_head, a->stride_qo_row, a->stride_qo_head, a->q_heads},
@@ -933,6 +934,7 @@ int dsa_v32_append_cache(const dsa_v32_append_args* a, void* stream) {
     if (a->num_tokens == 0) return DSA_V32_OK;
     if (!a->positions || !a->cos_sin || (a->kv && (!a->latent || !a->rope)) || (a->index_cache && !a->index_key)) return DSA_V32_ERR_NULL;
     if (a->index_bias && !a->index_weight) return DSA_V32_ERR_NULL;
+    if (a->index_cache && a->index_center && !a->index_weight) return DSA_V32_ERR_NULL;
     const int64_t unit = a->in_dtype == DSA_V32_DTYPE_FP32 ? 4 : 8;
     if (a->kv) {
         if (!strides_ok(a->num_tokens, a->stride_latent, 1, 0, kDV) || !strides_ok(a->num_tokens, a->stride_rope, 1, 0, kDRope)) return DSA_V32_ERR_SHAPE;

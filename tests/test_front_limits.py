@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 
 from opfoundry_b200 import api
-from test_front_args import BASE, NULL, SHAPE, append_args, refused
+from test_front_args import BASE, NULL, SHAPE, append_args, refused, rotate_args
 
 
 @pytest.mark.parametrize("rows", [650, 639, 1])
@@ -37,3 +37,15 @@ def test_topk_select_of_no_rows(built_lib):
     assert built_lib.dsa_v32_topk_select(None, 9, None, 0, 10, 4, None, None) == SHAPE
     for scores, out in ((None, BASE), (BASE, None)):
         assert built_lib.dsa_v32_topk_select(scores, 10, None, 1, 10, 4, out, None) == NULL
+
+
+def test_center_belongs_to_a_norm(built_lib):
+    """Without a weight there is no norm whose mean could be subtracted; the values would pass as they are."""
+    refused(built_lib.dsa_v32_norm_rotate, rotate_args, dict(center=1), NULL)
+    refused(built_lib.dsa_v32_norm_rotate, rotate_args, dict(center=1, k_weight=BASE), NULL)      # there are no keys
+    refused(built_lib.dsa_v32_append_cache, append_args, dict(index_center=1), NULL)
+    # (strides that are refused later: the call gets past the checks of the norm)
+    refused(built_lib.dsa_v32_norm_rotate, rotate_args, dict(center=1, q_weight=BASE, stride_q_head=120), SHAPE)
+    refused(built_lib.dsa_v32_norm_rotate, rotate_args, dict(center=1, k_weight=BASE, k_heads=1, k=BASE, k_out=BASE, stride_k_row=128, stride_ko_row=128, stride_q_head=120), SHAPE)
+    refused(built_lib.dsa_v32_append_cache, append_args, dict(index_center=1, index_weight=BASE, stride_index_key=120), SHAPE)
+    refused(built_lib.dsa_v32_append_cache, append_args, dict(index_center=1, index_cache=None, stride_latent=504), SHAPE)
