@@ -248,7 +248,7 @@ cudaError_t launch_block_select(const float* scores, int64_t stride_row, const i
     auto go = [&](auto kernel, int threads, int rows) {
         cudaLaunchConfig_t cfg = {};
         cudaLaunchAttribute attr[1];
-        cfg.gridDim = dim3((unsigned)((total_q + rows - 1) / rows), 1, 1);
+        cfg.gridDim = dim3((unsigned)(((int64_t)total_q + rows - 1) / rows), 1, 1);
         cfg.blockDim = dim3(threads, 1, 1);
         cfg.stream = stream;
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -29,3 +29,12 @@ def test_an_empty_step_of_single_positions(built_lib):
     q, pos = torch.empty(0, 4, 128, dtype=torch.bfloat16, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda")
     s = api.index_scores(q, torch.empty(0, 4, device="cuda"), api.index_cache_pages(2, False), pos, 128)
     assert s.shape == (0, 128) and api.topk_select(s, 16, pos).shape == (0, 16)
+
+
+def test_block_select_of_the_most_rows(built_lib):
+    """2^31 - 3 rows: rounded up to eight rows a CTA their number passes 31 bits."""
+    rows = 2 ** 31 - 3
+    s = torch.zeros(rows, 1, device="cuda")
+    out = torch.full((rows, 1), 7, dtype=torch.int32, device="cuda")
+    api.block_select(s, 1, 1, out=out)
+    assert not out.any()
