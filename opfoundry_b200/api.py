@@ -575,6 +575,7 @@ def index_scores(q, weights, index_cache, valid_len, kv_len, *, s_q=1, block=1, 
     kind, rows = _index_rows(index_cache, page_block_size)
     q0, q1, q2 = q.stride()
     w0, w1 = weights.stride()
+    assert kv_len > 0 and block > 0
     cols = -(-kv_len // block)
     if out is None:
         out = torch.empty(total_q, cols, dtype=_F32, device=q.device)
@@ -599,6 +600,7 @@ def block_select(scores, num_selected, block, valid_len=None, *, first=0, local=
     the num_selected best blocks of every row, the first `first` and last `local` ones always among them; ascending, -1 padded."""
     rows, blocks = scores.shape
     s0, s1 = scores.stride()
+    assert num_selected > 0 and block > 0
     if out is None:
         out = torch.empty(rows, num_selected * block, dtype=_I32, device=scores.device)
     assert scores.dtype is _F32 and (blocks == 1 or s1 == 1)

@@ -2,6 +2,7 @@
 import ctypes as C
 
 import pytest
+import torch
 
 from opfoundry_b200 import api
 from test_front_args import BASE, NULL, SHAPE, append_args, refused, rotate_args
@@ -49,3 +50,17 @@ def test_center_belongs_to_a_norm(built_lib):
     refused(built_lib.dsa_v32_norm_rotate, rotate_args, dict(center=1, k_weight=BASE, k_heads=1, k=BASE, k_out=BASE, stride_k_row=128, stride_ko_row=128, stride_q_head=120), SHAPE)
     refused(built_lib.dsa_v32_append_cache, append_args, dict(index_center=1, index_weight=BASE, stride_index_key=120), SHAPE)
     refused(built_lib.dsa_v32_append_cache, append_args, dict(index_center=1, index_cache=None, stride_latent=504), SHAPE)
+
+
+@pytest.mark.parametrize("kv_len,block", [(0, 1), (-5, 1), (64, 0), (64, -64)])
+def test_index_scores_of_no_columns(kv_len, block):
+    """Refused before the result's shape is formed from them."""
+    q, w, cache = torch.zeros(2, 4, 128, dtype=torch.bfloat16), torch.zeros(2, 4), torch.zeros(128, 128, dtype=torch.bfloat16)
+    with pytest.raises(AssertionError):
+        api.index_scores(q, w, cache, None, kv_len, block=block)
+
+
+@pytest.mark.parametrize("num_selected,block", [(0, 64), (-1, 64), (4, 0), (4, -1)])
+def test_block_select_of_no_positions(num_selected, block):
+    with pytest.raises(AssertionError):
+        api.block_select(torch.zeros(2, 10), num_selected, block)
