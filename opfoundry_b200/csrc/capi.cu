@@ -5,6 +5,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <vector>
 #include "defs.h"
@@ -876,6 +877,12 @@ int dsa_v32_pack_fp8_rows(const float* latent, const void* rope_bf16, const int6
 // ------------------------------------------------------------------ the front end
 namespace {
 bool misaligned(const void* p, uintptr_t mask) { return (reinterpret_cast<uintptr_t>(p) & mask) != 0; }
+// 4-byte words: an access off their boundary is a fault of the device
+bool words_misaligned(std::initializer_list<const void*> all) {
+    for (const void* p : all)
+        if (misaligned(p, 3)) return true;
+    return false;
+}
 
 // heads that do not overlap, rows likewise; a stride that no element uses may be anything
 bool strides_ok(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t dim) {
@@ -915,6 +922,7 @@ int dsa_v32_norm_rotate(const dsa_v32_norm_rotate_args* a, void* stream) {
         if (!strides_aligned(a->num_tokens, s.row, s.heads, s.head, in_unit) || !strides_aligned(a->num_tokens, s.o_row, s.heads, s.o_head, 8)) return DSA_V32_ERR_ALIGN;
     }
     if (misaligned(a->cos_sin, 15)) return DSA_V32_ERR_ALIGN;
+    if (words_misaligned({a->q_scale, a->k_scale, a->head_weight, a->positions})) return DSA_V32_ERR_ALIGN;
     cudaError_t e = launch_norm_rotate(*a, (cudaStream_t)stream);
     return e == cudaSuccess ? DSA_V32_OK : (int)e;
 }
@@ -946,7 +954,7 @@ int dsa_v32_append_cache(const dsa_v32_append_args* a, void* stream) {
         if (!aligned16(a->index_key) || !aligned16(a->index_cache) || misaligned(a->index_weight, 15) || misaligned(a->index_bias, 15)) return DSA_V32_ERR_ALIGN;
         if (!strides_aligned(a->num_tokens, a->stride_index_key, 1, 0, unit)) return DSA_V32_ERR_ALIGN;
     }
-    if (!aligned16(a->cos_sin)) return DSA_V32_ERR_ALIGN;
+    if (!aligned16(a->cos_sin) || words_misaligned({a->positions, a->seq_ids, a->block_table})) return DSA_V32_ERR_ALIGN;
     cudaError_t e = launch_append(*a, (cudaStream_t)stream);
     return e == cudaSuccess ? DSA_V32_OK : (int)e;
 }
@@ -966,7 +974,7 @@ int dsa_v32_index_scores(const dsa_v32_index_scores_args* a, void* stream) {
     if (!strides_ok(a->total_q, a->stride_q_row, a->H, a->stride_q_head, kDIndex)) return DSA_V32_ERR_SHAPE;
     if (a->total_q > 1 && (a->stride_w_row < a->H || a->stride_o_row < (a->kv_len + a->block - 1) / a->block)) return DSA_V32_ERR_SHAPE;
     if (!aligned16(a->q) || !aligned16(a->index_cache) || !strides_aligned(a->total_q, a->stride_q_row, a->H, a->stride_q_head, unit)) return DSA_V32_ERR_ALIGN;
-    if (misaligned(a->weights, 3) || misaligned(a->out, 3)) return DSA_V32_ERR_ALIGN;
+    if (words_misaligned({a->weights, a->out, a->valid_len, a->block_table, a->status})) return DSA_V32_ERR_ALIGN;
     // 16-byte rows of keys and heads: 128 bytes of a key and of a head are one row of a box
     const bool fp8 = a->cache_dtype == DSA_V32_KV_FP8;
     const uint64_t bytes = fp8 ? 1 : 2, page = uint64_t(a->page_block_size);
@@ -990,6 +998,7 @@ int dsa_v32_block_select(const float* scores, int64_t stride_row, const int32_t*
     if ((int64_t)num_blocks * block >= (int64_t(1) << 31) || (int64_t)num_selected * block >= (int64_t(1) << 31)) return DSA_V32_ERR_SHAPE;
     if (total_q == 0) return DSA_V32_OK;   // (empty tensors have no address)
     if (!scores || !indices_out) return DSA_V32_ERR_NULL;
+    if (words_misaligned({scores, valid_len, indices_out})) return DSA_V32_ERR_ALIGN;
     cudaError_t e = launch_block_select(scores, stride_row, valid_len, total_q, num_blocks, block, num_selected, first, local, indices_out, (cudaStream_t)stream);
     return e == cudaSuccess ? DSA_V32_OK : (int)e;
 }

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from opfoundry_b200 import api
-from test_front_args import BASE, NULL, SHAPE, append_args, refused, rotate_args
+from test_front_args import ALIGN, BASE, NULL, SHAPE, append_args, refused, rotate_args, scores_args
 
 
 @pytest.mark.parametrize("rows", [650, 639, 1])
@@ -64,3 +64,21 @@ def test_index_scores_of_no_columns(kv_len, block):
 def test_block_select_of_no_positions(num_selected, block):
     with pytest.raises(AssertionError):
         api.block_select(torch.zeros(2, 10), num_selected, block)
+
+
+@pytest.mark.parametrize("fn,make,fields", [("norm_rotate", rotate_args, ["q_scale", "k_scale", "head_weight", "positions"]), ("append_cache", append_args, ["positions", "seq_ids", "block_table"]),
+                                            ("index_scores", scores_args, ["valid_len", "block_table", "status", "weights", "out"])])
+def test_words_off_their_boundary_are_refused(built_lib, fn, make, fields):
+    for f in fields:
+        for off in (1, 2, 3):
+            changes = {f: BASE + off}
+            if f in ("q_scale", "k_scale", "head_weight"):
+                changes = dict(out_dtype=2, q_scale=BASE, k_heads=1, k=BASE, k_out=BASE, k_scale=BASE, stride_k_row=128, stride_ko_row=128) | changes
+            refused(getattr(built_lib, "dsa_v32_" + fn), make, changes, ALIGN)
+
+
+def test_block_select_refuses_words_off_their_boundary(built_lib):
+    for at in (0, 2, 9):
+        args = [BASE, 10, BASE, 1, 10, 64, 4, 0, 0, BASE]
+        args[at] = BASE + 2
+        assert built_lib.dsa_v32_block_select(*args, None) == ALIGN
