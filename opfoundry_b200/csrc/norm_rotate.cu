@@ -454,9 +454,12 @@ template <typename In, bool kE4m3> cudaError_t launch_rotate(RotateParams& p, in
     int sms = 0;
     cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) return e;
-    // Four heads a unit once there are threads enough for the device without (2048 an SM).
+    // Four heads a unit once there are threads enough for the device without (2048 an SM) and more than half of the units' places have a head.
+    // us with four and with one, normed heads of 128 in halves: 300 tokens x 17 heads (82 thousand threads) 3.5 and 2.8, 1000 x 17 (272 thousand) 4.4
+    // and 4.6, 4096 x 17 10.1 and 13.1, 4091 x 72 30.3 and 51.6; 40000 tokens of one head 14.0 and 8.0, of two 14.6 and 14.4, of three 15.9 and 21.2.
     auto go = [&](auto one, auto four, int lanes, int threads) {
-        const bool many = four != nullptr && tokens * p.heads * lanes >= (int64_t)sms * 2048;
+        const int of_four = (p.q_heads + 3) / 4 + (p.heads - p.q_heads + 3) / 4;
+        const bool many = four != nullptr && tokens * p.heads * lanes >= (int64_t)sms * 2048 && p.heads > 2 * of_four;
         const int each = many ? 4 : 1;
         p.q_chunks = (p.q_heads + each - 1) / each;
         p.chunks = p.q_chunks + (p.heads - p.q_heads + each - 1) / each;

@@ -30,3 +30,21 @@ def test_norm_on_one_side(built_lib, D, R, begin, T, H, Hk, side, center, fp8):
             check_e4m3(r[i].cpu(), r[2 + i].cpu()[..., None], y, m, D)
         else:
             check_bf16(r[i].cpu(), y, m)
+
+
+@pytest.mark.parametrize("H,Hk", [(1, 0), (1, 1), (2, 0), (3, 0), (5, 1)])
+def test_few_heads_of_many_tokens(built_lib, H, Hk):
+    """One head a unit or four, by how many places of four have a head: the bits of a call of few tokens."""
+    g = torch.Generator()
+    g.manual_seed(H)
+    T, P = 30000, 128
+    table, pos = rope_table(64, P).cuda(), torch.randint(0, P, (T,), generator=g).to(torch.int32).cuda()
+    q, k = torch.randn(T, H, 128, generator=g).bfloat16().cuda(), torch.randn(T, Hk, 128, generator=g).bfloat16().cuda() if Hk else None
+    w = (1 + 0.2 * torch.randn(128, generator=g)).cuda()
+    at = slice(29950, 30000)
+    for fp8 in (False, True):
+        args = dict(q_weight=w, k_weight=w if Hk else None, center=True, interleaved=False, out_dtype=E4M3 if fp8 else torch.bfloat16)
+        whole = api.norm_rotate(q, table, pos, k=k, **args)
+        few = api.norm_rotate(q[at], table, pos[at], k=None if k is None else k[at], **args)
+        for a, b in zip(whole, few):
+            assert (a is None) == (b is None) and (a is None or torch.equal(a[at].view(torch.uint8), b.view(torch.uint8)))
