@@ -707,15 +707,16 @@ cudaError_t launch_index_scores(const dsa_v32_index_scores_args& a, const CUtens
     while ((1 << p.block_shift) < a.block) ++p.block_shift;
     p.cols = (a.kv_len + a.block - 1) / a.block;
     p.block_table_stride = a.block_table_stride;
-    // Query rows of a group: 512 columns' worth where a sequence fills most of them, else up to 256 in groups of equal size (a group of
-    // 512 reads the keys half as often, but takes two full accumulators of every tile however many rows there are).
-    const int most = kTmemCols / cols;
-    const bool wide = 4 * a.s_q >= 3 * most;
-    p.per = most;
-    if (!wide) {
-        const int n = (a.s_q + most / 2 - 1) / (most / 2);
-        p.per = (a.s_q + n - 1) / n;
-    }
+    // Query rows of a group: 512 columns' worth, or up to 256 in groups of equal size.  A group of 512 reads the keys half as often, but takes two
+    // full accumulators of every tile however many rows there are: its time is that of about 0.6 of its rows in groups of 256, so wide groups it is
+    // where all narrow ones' rows are more than 0.6 of all wide ones' places.
+    // us wide and narrow, fp8, 16384 positions, 64 heads: 64 sequences of 3 rows 80 and 59, 4 82 and 76, 5 83 and 106, 6 84 and 107, 7 85 and 136, 8 86
+    // and 138; 16 sequences of 9 rows 49 and 44, 10 49 and 56, 16 50 and 72 (bf16 9 rows 53 and 46, 10 53 and 59).  32 heads: 64 sequences of 8 rows 85
+    // and 75, 9 86 and 93; 16 of 18 rows 50 and 47, 19 50 and 53.  16 heads: 16 of 18 rows 38 and 37, 19 39 and 40, 36 67 and 64, 40 67 and 73.
+    const int most = kTmemCols / cols, wide_groups = (int)(((int64_t)a.s_q + most - 1) / most), narrow_groups = (int)(((int64_t)a.s_q + most / 2 - 1) / (most / 2));
+    const int narrow_per = (int)(((int64_t)a.s_q + narrow_groups - 1) / narrow_groups);
+    const bool wide = 5 * (int64_t)narrow_groups * narrow_per > 3 * (int64_t)wide_groups * most;
+    p.per = wide ? most : narrow_per;
     p.groups_per_seq = (a.s_q + p.per - 1) / p.per;
     const int64_t groups = (int64_t)p.groups_per_seq * (a.total_q / a.s_q);
     p.acc_cols = 64;
