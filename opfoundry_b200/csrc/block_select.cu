@@ -8,9 +8,10 @@
 // every selected block its place; then the whole team writes the positions, 16 bytes at a time.
 //
 // A team of one warp takes a row of up to 512 blocks, of a CTA a longer one: up to 8 warps x 32 lanes x 32 keys, or 32 x 32 x 16; rows of
-// more blocks are read again for every trial.  The bytes (scores once, lists once) bound many rows, the chain of trials (about 13, one
-// exchange each) and the launch a few.  Measured against a CTA a row that read the scores for each of 32 trials and wrote from the selecting
-// threads: 4096 rows of 256 blocks to 2048 positions 105 us before, 64 rows of 2048 blocks 31 us.
+// more blocks are read again for every trial.  Bounds: the chain of trials (about 13, one exchange each), for many rows of up to 512 blocks beside the
+// bytes (scores once, lists once).  In a graph, inputs past L2, lists of 2048 positions: 64 rows of 2048 blocks 4.8 us, of 40000 80; 4096 rows of 256
+// blocks 10.4 (57 % of a copy's rate), of 512 15.5, of 1024 45, of 2048 47 (floor 9.1): every trial compares all keys of the row, 88 % of the issue slots.
+// A CTA a row that read the scores for each of 32 trials and wrote from the selecting threads took 105 us for 4096 rows of 256 blocks and 31 for 64 of 2048.
 #include "front.h"
 #include "ptx.cuh"
 

@@ -8,11 +8,13 @@
 // Roles of a CTA (one an SM): warps 0-15 take the scores out of TMEM (four warpgroups, a query row at a time each), warp 16 brings tiles
 // of 128 keys page by page (TMA; an fp8 cache's scales by bulk copies), warp 17 the query rows, their weights and lengths, warp 18
 // issues the MMAs.  A work item is tiles of a group of query rows of one sequence.  The tiles that the rows see are dealt out evenly over the CTAs
-// (up to 1024 groups; more take chunks in turn: 64 sequences of 16384 to 32768 positions x 2 rows took 66 instead of 47 us that way), and columns
-// that no row sees are filled by warps that have nothing else to do.
+// (up to kDealt groups; more take chunks in turn), and columns that no row sees are filled by warps that have nothing else to do.
 //
-// Bounds: decode HBM (fp8: 64 x 2 rows, 53 us for 208 MB), long chunks the power cap (4096 rows over 16384 positions: 515 us in a short run, 590 in a
-// long one at 1.72 GHz; bf16 637 and 745), where the MMAs take two fifths of the cycles and the sums over heads two thirds of the issue slots.
+// Bounds (64 heads; times in a graph, inputs past L2): decode HBM and about 6 us that are fixed (fp8: 64 x 2 rows of 16384 to 32768 positions, 208 MB,
+// 48 us; 56 as a call among others; bf16: 73).  Chunks: the drain of the accumulators.  4096 rows over 16384 positions take 515 us in bursts of 40 ms
+// (1.965 GHz) and 591 back to back for seconds, where the power cap holds 1.717 GHz: 1.01 million cycles either way, of which the fp8 MMAs use two
+// fifths and the sums over heads two thirds of the issue slots, so neither is full; a warpgroup loads, waits for and sums its rows one after the
+// other.  In bf16 the MMAs are the larger part: 656 and 747 us (at 1.425 GHz).
 #include <cuda_bf16.h>
 #include <cstddef>
 #include <mutex>
@@ -32,7 +34,12 @@ constexpr int kMaxStages = 12;
 constexpr int kMaxSlots = 8;
 constexpr int kSmemBytes = 227 * 1024;
 constexpr int kScaleBytes = kTile * 4;
-constexpr int kDealt = 1024;          // most groups whose tiles are dealt out evenly
+// Most groups whose tiles are dealt out evenly.  us dealt and in turn, 64 heads, fp8, ragged lengths from a half of the longest on: 64 x 2 rows to
+// 32768 positions 48 and 56, 256 sequences to 8192 44 and 50, 1000 to 4096 84 and 93, 4096 rows over 16384 516 and 545.  It costs every CTA a pass
+// over the lengths: one sequence 7.1 and 5.6 (but the lengths are not known here, and one far shorter than kv_len would keep a few CTAs busy only),
+// 1100 sequences to 200 positions 24 and 19, 2000 to 512 39 and 37, 10000 to 1000 253 and 230.  Between 1024 and 4096 groups of many tiles it would
+// still gain (2500 to 4096: 199 and 222).
+constexpr int kDealt = 1024;
 
 struct Control {
     uint64_t k_full[kMaxStages], k_empty[kMaxStages];
@@ -234,8 +241,8 @@ __device__ __forceinline__ void fill_unseen(const Params& p, Control* ctl, int l
 // d[4 i], d[4 i + 1] and of lane t / 4 + 8 in d[4 i + 2], d[4 i + 3].  So a thread needs the weights of a quarter of the heads only (all of
 // them for every position, read from shared memory for every accumulator, were as many wavefronts as the MMAs' own operands and kept the
 // kernel at 1 800 cycles an accumulator), and the four threads of a quad add up their parts for four positions.
-// The loads and their wait are one statement: with code between them (scores of the row before on their way out) an accumulator that was given back
-// behind the wait was overwritten before its upper half had been read.
+// The loads and their wait are one statement, as the sums read nothing but registers: with a wait of its own nothing would keep them behind it.
+// (Apart, with the scores of the row before on their way out in between, some sums were wrong.)
 template <int kCols> __device__ __forceinline__ void load_row(uint32_t taddr, uint32_t (&lo)[kCols / 2], uint32_t (&hi)[kCols / 2]) {
     if constexpr (kCols == 64) {
         asm volatile(
@@ -284,8 +291,8 @@ __device__ __forceinline__ int lane_position(int lane) { return (lane >> 2) + 8 
 __device__ __forceinline__ int lane_of_offset(int off) { return off < 8 ? 4 * off : off >> 3; }
 
 // The sum of w_h max(0, d_h) over a pair of heads is two maxima (half rate) and two multiply-adds.  With max(0, d) taken as (d + |d|) / 2 it is a
-// two-wide multiply-add and two with |d|, three instructions: within 1 % for 4096 rows over 16384 positions (510 to 512 us) and slower for 64 x 2 rows
-// over 32768 (71.7 instead of 69.1), so it stays out.
+// two-wide multiply-add and two with |d|, three instructions: when it was tried, within 1 % for 4096 rows over 16384 positions and 4 % slower for 64 x 2
+// rows over 32768, so it stays out.
 struct Sum {
     float a = 0.0f, b = 0.0f;
     __device__ __forceinline__ void add(uint32_t d0, uint32_t d1, float u, float v) {

@@ -2,9 +2,11 @@
 //
 // A vector x of one head (or one latent): with mu its mean (0 unless centred), y = (x - mu) / sqrt(mean((x - mu)^2) + eps) * w + b, then
 // pairs of its rotated values turned by the angle of the token's position, then one rounding to bf16, or to e4m3 with scale = amax / 448.
-// Everything between the load and that rounding is fp32.  Bound by HBM: every value is read and written once (4091 tokens of 64 + 8 heads of 128 in
-// 31 us, 4.9 TB/s); a few tokens by the launch (1.7 us in a graph), and appends by their chain position -> page -> row (64 tokens 2.4 us, 16384 into the
-// fp8 caches 12.5).
+// Everything between the load and that rounding is fp32.  Every value is read and written once.  Times in a graph, inputs of many tokens past L2:
+// 4091 tokens of 64 + 8 heads of 128, bf16 to bf16, 30 us (5.0 TB/s, 78 % of a copy), bound by HBM; 4096 x 64 heads to e4m3 30 us (3.3 TB/s), bound by
+// loads and the chain of largest value, scale and quotients behind them (62 % of the issue slots); 4096 x 8 heads of 576 37 us (2.1 TB/s), by loads that
+// 16 warps an SM have in flight (93 registers).  A few tokens are bound by the launch (1.7 us), appends by their chain position -> page -> row (64 tokens 2.4 us, 16380 into the fp8 caches
+// 16.4, 12.6 with inputs in L2).
 #include <cuda_bf16.h>
 #include <type_traits>
 #include "front.h"
@@ -144,9 +146,9 @@ __device__ __noinline__ uint2 divide8(float a, float b, float c, float d, float 
     return make_uint2(e4m3x4(__fdiv_rn(a, scale), __fdiv_rn(b, scale), __fdiv_rn(c, scale), __fdiv_rn(d, scale)),
                       e4m3x4(__fdiv_rn(e, scale), __fdiv_rn(f, scale), __fdiv_rn(g, scale), __fdiv_rn(h, scale)));
 }
-// Eight values over their scale as e4m3, each the rounded quotient (one step of Newton and one of Markstein, as in merge_pack.cu), two at a time.
+// Eight values over their scale as e4m3, each the rounded quotient (one step of Markstein, as in merge_pack.cu), two at a time.
 // n: the values negated, so that a zero keeps its sign: q = n (-1/s), then q - (q s + n) / s.  (Products with 1 / s alone give another
-// code at some ties: 27.8 instead of 29.4 us for 4096 x 64 heads of 128.)
+// code at some ties, in 5 % less time for 4096 x 64 heads of 128.)
 __device__ __forceinline__ uint2 quotients8(const uint64_t (&n)[4], float scale) {
     if (!(scale >= 0x1p-80f && scale <= 0x1p80f)) {
         float v[8];
@@ -709,7 +711,7 @@ template <typename In, bool kFp8, int kTokens> __device__ __forceinline__ void a
     }
 }
 
-// (Blocks of 256 threads: 14.8 instead of 12.5 us for 16384 tokens into the fp8 caches, the last ones leave SMs half empty.)
+// (Blocks of 256 threads: 14.8 instead of 12.5 us for 16384 tokens into the fp8 caches, inputs in L2: the last ones leave SMs half empty.)
 constexpr int kAppendThreads = 128;
 // Warps 0 .. latent_warps - 1 take kTokens tokens' rows of the attention's cache each, the others twice as many (at least two) of the index cache.
 template <typename In, bool kFp8, int kTokens>
@@ -779,7 +781,7 @@ cudaError_t launch_append(const dsa_v32_append_args& a, cudaStream_t stream) {
         return launch_after(kernel, (warps + kAppendThreads / 32 - 1) / (kAppendThreads / 32), kAppendThreads, p, stream);
     };
     // Two tokens a warp (their loads in flight together, the weights read once) where warps of one token each are more than the device holds with
-    // their CTAs' ends: 4096 tokens 4.8 instead of 5.6 us, 1024 tokens 3.4 instead of 2.9.  (Four: 14.2 instead of 12.5 us for 16384 tokens.)
+    // their CTAs' ends: inputs in L2, 4096 tokens 4.8 instead of 5.6 us, 1024 tokens 3.4 instead of 2.9.  (Four: 14.2 instead of 12.5 us for 16384 tokens.)
     if (a.num_tokens < 16 * sms) {
         if (wide) return fp8 ? go(append_kernel<float, true, 1>, 1) : go(append_kernel<float, false, 1>, 1);
         return fp8 ? go(append_kernel<__nv_bfloat16, true, 1>, 1) : go(append_kernel<__nv_bfloat16, false, 1>, 1);
