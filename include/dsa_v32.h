@@ -374,6 +374,7 @@ int dsa_v32_pack_fp8_rows(const float* latent, const void* rope_bf16, const int6
  * weight + bias; a NULL weight means no norm (so no centring) of those vectors, a NULL bias none.  A bias without its weight, and
  * `center` where nothing has a weight, are refused.  Values are rounded once, at the end.
  * e4m3 outputs: scale = amax / 448 (1 for a vector of zeros), value = e4m3(x / scale), as in dsa_v32_pack_fp8_rows.
+ * Addresses of 4-byte words that no other boundary is given for are multiples of 4.
  */
 #define DSA_V32_DTYPE_BF16 0
 #define DSA_V32_DTYPE_FP32 1
@@ -422,8 +423,9 @@ int dsa_v32_norm_rotate(const dsa_v32_norm_rotate_args* args, void* stream);
  * row of the attention's cache is the normed latent (512 values) beside the rotated rope key (64 values); its row of the
  * index cache the normed index key (128 values) whose first 64 are rotated.  Either cache may be left out (kv / index_cache
  * NULL).  A token whose sequence is negative, whose position is outside the table, or whose row lies outside the cache (without a
- * block table: outside its sequence's kv_batch_stride_rows rows, when those are not 0) is not written; no other byte of the caches changes.  A (sequence, position) may occur once in a call.  The rows of the inputs
- * start on 16-byte boundaries.
+ * block table: outside its sequence's kv_batch_stride_rows rows, when those are not 0) is not written; no other byte of the caches changes.  A row
+ * may be written once in a call: no (sequence, position) twice, nor one page or (kv_batch_stride_rows 0) one row of two sequences.  The rows of the
+ * inputs start on 16-byte boundaries.
  */
 typedef struct dsa_v32_append_args {
     const void* latent;        /* [num_tokens, 512], row stride below; in_dtype */
